@@ -708,6 +708,127 @@ typedef struct {
 size_t smoe_layer_backward_scratch_size(int T, int H, int I, int E, int K);
 int smoe_layer_backward(const smoe_layer_bwd* args, void* stream, void* side_stream);
 
+/* ------------------------------------------------------------------------
+ * Operators of an unquantised expert block.  Element types are SMOE_BF16,
+ * SMOE_F16 and SMOE_F32; a tensor may start at any multiple of its element
+ * size, and "ld" arguments are the elements between an input's rows (outputs
+ * and weights are dense).  Row lengths need not be multiples of anything.
+ * No counterpart in the reference beyond the dataflow each one serves:
+ * dispatch and combine (moe/MoE_detailed_computation_dataflow.md:94-116,195),
+ * expert products (moe/MegatronCore_MoE_reading_notes.md:84-116).
+ */
+#define SMOE_BF16 0
+#define SMOE_F16 1
+#define SMOE_F32 2
+
+/*
+ * Token rows to expert rows and back.  inv_map [T*K] as the sort gives it; a
+ * pair whose entry lies outside [0, T*K) has no row: nothing is read or
+ * written for it.  w [T,K] f32, or NULL for no weights.
+ *   permute_tokens        xp[inv] = w x[t]                 (rows without a pair unwritten)
+ *   permute_tokens_bwd    dx[t] = sum_k w dxp[inv],  dw[t,k] = <x[t], dxp[inv]>
+ *   unpermute_tokens      out[t] = sum_k w y[inv]
+ *   unpermute_tokens_bwd  dy[inv] = w dout[t],       dw[t,k] = <dout[t], y[inv]>
+ * dw [T,K] f32 may be NULL (then x or y is not read and may be NULL too).
+ * Sums are fp32 in k order, rounded once.  K <= 32.
+ */
+int smoe_permute_tokens(const void* x, long long ldx, const int32_t* inv_map, const float* w,
+                        int T, int K, int H, int dtype, void* xp, void* stream);
+int smoe_permute_tokens_bwd(const void* dxp, long long lddxp, const void* x, long long ldx,
+                            const int32_t* inv_map, const float* w, int T, int K, int H, int dtype,
+                            void* dx, float* dw, void* stream);
+int smoe_unpermute_tokens(const void* y, long long ldy, const int32_t* inv_map, const float* w,
+                          int T, int K, int H, int dtype, void* out, void* stream);
+int smoe_unpermute_tokens_bwd(const void* dout, long long lddout, const void* y, long long ldy,
+                              const int32_t* inv_map, const float* w, int T, int K, int H,
+                              int dtype, void* dy, float* dw, void* stream);
+
+/*
+ * RMS norms before and after a block, H <= 65536.
+ *   block_norm_in   h = x rstd weight,  rstd [T] f32 = 1 / sqrt(mean(x^2) + eps), eps > 0
+ *   block_norm_out  out = residual_scale x + gate (y rstd weight), rstd of y
+ * weight [H] may be NULL (ones).  gate_mode: SMOE_GATE_NONE; _CHANNEL, gate
+ * [H]; _TOKEN, gate [T] (ldgate apart); _FULL, gate [T,H].  param_f32 bit 0:
+ * weight (and dweight) are f32 instead of dtype, bit 1: gate (and dgate).
+ * The gradients, with n = (x or y) rstd:
+ *   block_norm_in_bwd   dx = rstd (c - n mean(c n)) + skip_scale dskip, c = dh weight
+ *                       (dskip NULL: without), dweight = sum_t dh n
+ *   block_norm_out_bwd  dy likewise from c = dout gate weight, dweight =
+ *                       sum_t dout gate n, dgate = dout n weight summed over
+ *                       what the gate was broadcast along; the residual's own
+ *                       gradient is residual_scale dout
+ * dweight may be NULL.  ws must hold smoe_block_norm_bwd_workspace_size()
+ * bytes where dweight or a channel gate's dgate is asked for.
+ */
+#define SMOE_GATE_NONE 0
+#define SMOE_GATE_CHANNEL 1
+#define SMOE_GATE_TOKEN 2
+#define SMOE_GATE_FULL 3
+int smoe_block_norm_in(const void* x, long long ldx, const void* weight, int param_f32, float eps,
+                       int T, int H, int dtype, void* h, float* rstd, void* stream);
+int smoe_block_norm_out(const void* y, long long ldy, const void* x, long long ldx,
+                        const void* weight, const void* gate, long long ldgate, int gate_mode,
+                        int param_f32, float residual_scale, float eps, int T, int H, int dtype,
+                        void* out, float* rstd, void* stream);
+size_t smoe_block_norm_bwd_workspace_size(int T, int H);
+int smoe_block_norm_in_bwd(const void* dh, long long lddh, const void* x, long long ldx,
+                           const float* rstd, const void* weight, int param_f32, const void* dskip,
+                           long long ldskip, float skip_scale, int T, int H, int dtype, void* dx,
+                           void* dweight, void* ws, size_t ws_bytes, void* stream);
+int smoe_block_norm_out_bwd(const void* dout, long long lddout, const void* y, long long ldy,
+                            const float* rstd, const void* weight, const void* gate,
+                            long long ldgate, int gate_mode, int param_f32, int T, int H, int dtype,
+                            void* dy, void* dweight, void* dgate, void* ws, size_t ws_bytes,
+                            void* stream);
+
+/*
+ * out = act(x W^T + bias) + residual in bf16 or fp16 (fp32 sums, rounded
+ * once).  w [N,K] with offsets NULL and E = 1, or [E,N,K] with offsets [E+1]
+ * over x's rows: expert e has rows [offsets[e], offsets[e+1]), clamped to
+ * [0, R); rows in no expert's range are not written.  act SMOE_ACT_SWIGLU
+ * takes W's rows as gate | up halves: out = silu(gate) up, N/2 columns.
+ * z [R,N] (may be NULL) receives x W^T + bias for the backward pass.
+ * R <= 2^29, N and K <= 2^20.
+ *
+ * The gradients, dz = dout act'(z) (z may be NULL for SMOE_ACT_NONE):
+ * dx = dz W, dw = dz^T x per expert, dbias = sum of dz; each output may be
+ * NULL.  dz is rounded to dtype as the products' operand.  dw_mode is one of
+ * SMOE_WGRAD_F32 ... SMOE_WGRAD_BF16_ACC ("BF16" reads: dtype).  An expert
+ * without rows gets zero gradients (accumulating modes: leaves dw as it is).
+ * The residual's gradient is dout.
+ */
+#define SMOE_ACT_NONE 0
+#define SMOE_ACT_RELU 1
+#define SMOE_ACT_SILU 2
+#define SMOE_ACT_GELU 3
+#define SMOE_ACT_GELU_TANH 4
+#define SMOE_ACT_SWIGLU 5
+typedef struct {
+  int R, N, K, E, act, dtype, bias_f32;
+  const void* x;
+  long long ldx;
+  const void *w, *bias, *residual;
+  long long ldr;
+  const int32_t* offsets;
+  void *out, *z, *ws;
+  size_t ws_bytes;
+} smoe_linear_fwd;
+typedef struct {
+  int R, N, K, E, act, dtype, bias_f32, dw_mode;
+  const void* dout;
+  long long lddout;
+  const void* x;
+  long long ldx;
+  const void *w, *z;
+  const int32_t* offsets;
+  void *dx, *dw, *dbias, *ws;
+  size_t ws_bytes;
+} smoe_linear_bwd;
+size_t smoe_linear_act_workspace_size(int R, int N, int K, int E, int act);
+int smoe_linear_act(const smoe_linear_fwd* args, void* stream);
+size_t smoe_linear_act_bwd_workspace_size(int R, int N, int K, int E, int act, int with_bias);
+int smoe_linear_act_bwd(const smoe_linear_bwd* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,447 @@
+// smoe_linear.hip — matrix products with bias, activation and residual in the
+// epilogue, dense or one weight per expert, and their gradients (gfx950).
+//
+//   out = act(x W^T + b) + residual          x [R, K], W [N, K] or [E, N, K]
+//   dz  = dout act'(z),  db = sum of dz over rows
+//   dx  = dz W,          dW = dz^T x
+//
+// Products are bf16 or fp16 MFMA with fp32 accumulators; bias, activation and
+// residual are applied to the fp32 sum and rounded once.  dz is kept in the
+// operands' 16-bit type: it is the MFMA operand of both gradients (one
+// rounding of 2^-9 relative on average, below that of dx and dW themselves).
+#include "smoe_linear.h"
+
+namespace smoe {
+
+constexpr int kLinearMaxDim = 1 << 20, kLinearMaxRows = 1 << 29;
+
+// ------------------------------------------------ the product, any sizes ---
+// 64 x 64 tiles, 4 waves of 32 x 32, K in steps of 32 staged through LDS by
+// way of registers.  Rows and columns of any length and alignment.
+enum { kFwd = 0, kDgrad = 1, kWgrad = 2 };
+constexpr int kT = 64, kTK = 32, kPitch = kTK + 8;  // LDS row pitch: 80 bytes
+
+// 8 elements of a row, those past n read as 0 (n may be <= 0).
+template <class T>
+__device__ __forceinline__ v4u_t piece_or_zero(const T* p, int n) {
+  if (n >= 8) return load_piece<T>(p);
+  struct { T v[8]; } b;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b.v[i] = i < n ? p[i] : T{};
+  return __builtin_bit_cast(v4u_t, b);
+}
+
+// One lane's four neighbouring outputs n .. n + 3 of row m.
+template <class T>
+__device__ __forceinline__ void store4(T* p, int n, const float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) p[i] = Elt<T>::from_f32(f[i]);
+}
+template <class T>
+__device__ __forceinline__ float bias_at(const LinArgs& a, size_t i) {
+  return a.bias_f32 ? ((const float*)a.bias)[i] : Elt<T>::to_f32(((const T*)a.bias)[i]);
+}
+
+template <class T, int kAct>
+__device__ __forceinline__ void epilogue4(const LinArgs& a, int e, int m, int n, int cols, float* v, const float* u) {
+  // v: values n .. n+3 of row m (SwiGLU: the gate's, u: the up's), cols: the
+  // output's row length
+  const int left = cols - n;
+  if (left <= 0) return;
+  const size_t nb = (size_t)e * a.N + n;
+  if (a.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) v[i] = v[i] + bias_at<T>(a, nb + i);
+  }
+  float o[4];
+  if constexpr (kAct == SMOE_ACT_SWIGLU) {
+    float w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = u[i];
+      if (a.bias && i < left) w[i] = w[i] + bias_at<T>(a, nb + cols + i);
+      o[i] = act_value<SMOE_ACT_SILU>(v[i]) * w[i];
+    }
+    if (a.z) {
+      store4<T>((T*)a.z + (size_t)m * a.N + n, left, v);
+      store4<T>((T*)a.z + (size_t)m * a.N + cols + n, left, w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = act_value<kAct>(v[i]);
+    if (a.z) store4<T>((T*)a.z + (size_t)m * a.N + n, left, v);
+  }
+  if (a.residual) {
+    const T* r = (const T*)a.residual + (long long)m * a.ldr + n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) o[i] = o[i] + Elt<T>::to_f32(r[i]);
+  }
+  store4<T>((T*)a.out + (size_t)m * cols + n, left, o);
+}
+
+// kFwd:   D[m][n] = sum_k x[m][k] W[n][k]         rows of the tile's expert
+// kDgrad: D[m][k] = sum_n dz[m][n] W[n][k]        "
+// kWgrad: D[n][k] = sum_r dz[r][n] x[r][k]        over the expert's rows
+// Left and right tiles lie in LDS with the summed index contiguous; operands
+// whose rows run along the other index are turned on the way in.
+template <class T, int kWhat, int kAct>
+__global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a) {
+  __shared__ __attribute__((aligned(16))) T left[kT * kPitch], right[kT * kPitch];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
+  constexpr bool kPair = kWhat == kFwd && kAct == SMOE_ACT_SWIGLU;
+  const int half = a.N / 2;
+  int e = 0, m0, mrows, n0 = blockIdx.y * kT, ncols, len, k_lo = 0;
+  if constexpr (kWhat == kWgrad) {
+    e = blockIdx.z;
+    m0 = blockIdx.x * kT;
+    mrows = a.N - m0;
+    ncols = a.K;
+    int lo = 0, hi = a.R;
+    if (a.offsets) {
+      lo = clamp_row(a.offsets, e, a.R);
+      hi = clamp_row(a.offsets, e + 1, a.R);
+    }
+    k_lo = lo;
+    len = hi > lo ? hi - lo : 0;
+    if (len == 0 && (a.mode & 1)) return;  // nothing to add
+  } else {
+    RowTile t;
+    if (!find_row_tile<kT>(a.offsets, a.E, a.R, blockIdx.x, &t)) return;
+    e = t.e;
+    m0 = t.row0;
+    mrows = t.rows;
+    ncols = kWhat == kFwd ? (kPair ? half : a.N) : a.K;
+    len = kWhat == kFwd ? a.K : a.N;
+    if (kPair) n0 = blockIdx.y * (kT / 2);
+  }
+  const T* A = (const T*)a.a;
+  const T* B = (const T*)a.b + (kWhat == kWgrad ? 0 : (size_t)e * a.N * a.K);
+  v4f_t acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (int k0 = 0; k0 < len; k0 += kTK) {
+    // 64 rows x 32 k a tile: 256 pieces of 8, one a thread
+    const int r = tid >> 2, c = (tid & 3) * 8;       // row-wise: row r, k = c ..
+    const int kr = tid >> 3, cr = (tid & 7) * 8;     // turned: k = kr, rows cr ..
+    v4u_t pa, pb;
+    if constexpr (kWhat != kWgrad) {
+      const int row = r < mrows ? m0 + r : m0;
+      pa = piece_or_zero<T>(A + (long long)row * a.lda + k0 + c, r < mrows ? len - k0 - c : 0);
+    } else {
+      const int row = k_lo + (k0 + kr < len ? k0 + kr : 0);
+      pa = piece_or_zero<T>(A + (long long)row * a.lda + m0 + cr, k0 + kr < len ? mrows - cr : 0);
+    }
+    if constexpr (kWhat == kFwd) {
+      int n = n0 + r, ok = n < ncols;
+      if constexpr (kPair) {  // 16 gate rows, 16 up rows, alternately
+        n = n0 + (r >> 5) * 16 + (r & 15);
+        ok = n < half;
+        n += (r & 16) ? half : 0;
+      }
+      pb = piece_or_zero<T>(B + (size_t)(ok ? n : 0) * a.K + k0 + c, ok ? len - k0 - c : 0);
+    } else if constexpr (kWhat == kDgrad) {
+      const int n = k0 + kr;
+      pb = piece_or_zero<T>(B + (size_t)(n < len ? n : 0) * a.K + n0 + cr, n < len ? ncols - n0 - cr : 0);
+    } else {
+      const int row = k_lo + (k0 + kr < len ? k0 + kr : 0);
+      pb = piece_or_zero<T>(B + (long long)row * a.ldb + n0 + cr, k0 + kr < len ? ncols - n0 - cr : 0);
+    }
+    __syncthreads();
+    auto turn = [&](T* t, const v4u_t& p) {
+      struct B { T v[8]; };
+      const B b = __builtin_bit_cast(B, p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[(cr + i) * kPitch + kr] = b.v[i];
+    };
+    if constexpr (kWhat != kWgrad) *(v4u_t*)(left + r * kPitch + c) = pa;
+    else turn(left, pa);
+    if constexpr (kWhat == kFwd) *(v4u_t*)(right + r * kPitch + c) = pb;
+    else turn(right, pb);
+    __syncthreads();
+    v4u_t fa[2], fb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      fa[i] = *(const v4u_t*)(left + (wm + i * 16 + (lane & 15)) * kPitch + (lane >> 4) * 8);
+      fb[i] = *(const v4u_t*)(right + (wn + i * 16 + (lane & 15)) * kPitch + (lane >> 4) * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = mfma32<T>(fb[j], fa[i], acc[i][j]);
+  }
+
+  // the right operand went in first: a lane holds four neighbouring columns
+  const int mi = lane & 15, nq = (lane >> 4) * 4;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int m = wm + i * 16 + mi;
+    if (m >= mrows) continue;
+    if constexpr (kWhat == kFwd) {
+      if constexpr (kPair) {
+        epilogue4<T, kAct>(a, e, m0 + m, n0 + wn / 2 + nq, half, (float*)&acc[i][0], (const float*)&acc[i][1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          epilogue4<T, kAct>(a, e, m0 + m, n0 + wn + j * 16 + nq, a.N, (float*)&acc[i][j], nullptr);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = n0 + wn + j * 16 + nq;
+        const int n_left = ncols - n;
+        if (n_left <= 0) continue;
+        float* v = (float*)&acc[i][j];
+        if constexpr (kWhat == kDgrad) {
+          store4<T>((T*)a.out + (size_t)(m0 + m) * a.K + n, n_left, v);
+        } else {
+          const size_t at = ((size_t)e * a.N + m0 + m) * a.K + n;
+          if (a.mode < 2) {
+            float* d = (float*)a.out + at;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (q < n_left) d[q] = (a.mode & 1) ? d[q] + v[q] : v[q];
+          } else {
+            T* d = (T*)a.out + at;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (q < n_left) d[q] = Elt<T>::from_f32((a.mode & 1) ? Elt<T>::to_f32(d[q]) + v[q] : v[q]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------- dz and the biases' gradient ---
+// Rows in blocks of 64 of one expert; a thread owns 8 columns (SwiGLU: 8 gate
+// columns and their 8 up columns), 32 threads side by side and 8 rows at a
+// time.  dz (unless NULL) is rounded to T; the column sums are of the fp32
+// values, one partial row a block.
+constexpr int kDzRows = 64;
+struct DzArgs {
+  const void *dout, *z;
+  void* dz;
+  float* part;  // [blocks, N], or NULL
+  const int32_t* offsets;
+  long long lddout;
+  int E, R, N;
+};
+
+template <class T, int kAct>
+__global__ __launch_bounds__(256) void linear_dz_kernel(const DzArgs a) {
+  constexpr bool kPair = kAct == SMOE_ACT_SWIGLU;
+  __shared__ float red[kPair ? 2 : 1][8][32][8 + 1];
+  RowTile t;
+  if (!find_row_tile<kDzRows>(a.offsets, a.E, a.R, blockIdx.x, &t)) return;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int M = kPair ? a.N / 2 : a.N, c = (blockIdx.y * 32 + tx) * 8, n = M - c;
+  float s0[8], s1[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s0[i] = s1[i] = 0.0f;
+  if (n > 0) {
+    for (int r = ty; r < t.rows; r += 8) {
+      const size_t row = (size_t)t.row0 + r;
+      float g[8], z[8];
+      load_f32<T>((const T*)a.dout + (long long)row * a.lddout + c, n, g);
+      if constexpr (kAct != SMOE_ACT_NONE) load_f32<T>((const T*)a.z + row * a.N + c, n, z);
+      if constexpr (kPair) {
+        float u[8], dg[8], du[8];
+        load_f32<T>((const T*)a.z + row * a.N + M + c, n, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float p = sigmoid_fast(z[i]);
+          dg[i] = g[i] * u[i] * (p * (1.0f + z[i] * (1.0f - p)));
+          du[i] = g[i] * (z[i] * p);
+          s0[i] = s0[i] + dg[i];
+          s1[i] = s1[i] + du[i];
+        }
+        if (a.dz) {
+          store_f32<T>((T*)a.dz + row * a.N + c, n, dg);
+          store_f32<T>((T*)a.dz + row * a.N + M + c, n, du);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (kAct != SMOE_ACT_NONE) g[i] = g[i] * act_slope<kAct>(z[i]);
+          s0[i] = s0[i] + g[i];
+        }
+        if (a.dz) store_f32<T>((T*)a.dz + row * a.N + c, n, g);
+      }
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    red[0][ty][tx][i] = s0[i];
+    if constexpr (kPair) red[1][ty][tx][i] = s1[i];
+  }
+  __syncthreads();
+  // thread: column threadIdx.x of the block's 256
+  const int col = blockIdx.y * 256 + threadIdx.x;
+  if (col >= M) return;
+#pragma unroll
+  for (int h = 0; h < (kPair ? 2 : 1); ++h) {
+    float s = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) s = s + red[h][y][threadIdx.x >> 3][threadIdx.x & 7];
+    a.part[(size_t)blockIdx.x * a.N + h * M + col] = s;
+  }
+}
+
+// db[e] = the sum of expert e's partial rows, in order.
+template <class T>
+__global__ __launch_bounds__(256) void linear_db_kernel(const float* part, const int32_t* offsets, int blocks, int R,
+                                                        int N, int f32, void* db) {
+  const int e = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+  int first = 0, count = (R + kDzRows - 1) / kDzRows;
+  if (offsets) {
+    // the blocks of the experts before e (every thread for itself: E is small);
+    // bounds out of order may count more blocks than there are
+    for (int i = 0; i <= e; ++i) {
+      int n = clamp_row(offsets, i + 1, R) - clamp_row(offsets, i, R);
+      count = n > 0 ? (n + kDzRows - 1) / kDzRows : 0;
+      if (i < e) first = first + count < blocks ? first + count : blocks;
+    }
+    if (count > blocks - first) count = blocks - first;
+  }
+  if (c >= N) return;
+  float s = 0.0f;
+  for (int b = 0; b < count; ++b) s = s + part[(size_t)(first + b) * N + c];
+  if (f32) ((float*)db)[(size_t)e * N + c] = s;
+  else ((T*)db)[(size_t)e * N + c] = Elt<T>::from_f32(s);
+}
+
+// ------------------------------------------------------------ launching ----
+static int row_tiles(int R, int E, int bm) { return (R + bm - 1) / bm + E - 1; }
+
+#define SMOE_LIN_ACTS(CALL)                                            \
+  do {                                                                 \
+    switch (act) {                                                     \
+      case SMOE_ACT_NONE: CALL(SMOE_ACT_NONE); break;                  \
+      case SMOE_ACT_RELU: CALL(SMOE_ACT_RELU); break;                  \
+      case SMOE_ACT_SILU: CALL(SMOE_ACT_SILU); break;                  \
+      case SMOE_ACT_GELU: CALL(SMOE_ACT_GELU); break;                  \
+      case SMOE_ACT_GELU_TANH: CALL(SMOE_ACT_GELU_TANH); break;        \
+      default: CALL(SMOE_ACT_SWIGLU); break;                           \
+    }                                                                  \
+  } while (0)
+
+template <class T>
+static int linear_fwd(const LinArgs& a, hipStream_t s) {
+  const int act = a.act;
+  const int cols = act == SMOE_ACT_SWIGLU ? a.N / 2 : a.N, bn = act == SMOE_ACT_SWIGLU ? kT / 2 : kT;
+  const dim3 grid(row_tiles(a.R, a.E, kT), (cols + bn - 1) / bn);
+#define SMOE_LF(A) linear_any_kernel<T, kFwd, A><<<grid, dim3(256), 0, s>>>(a)
+  SMOE_LIN_ACTS(SMOE_LF);
+#undef SMOE_LF
+  SMOE_RETURN_LAUNCH();
+}
+
+template <class T>
+static int linear_bwd(const smoe_linear_bwd& q, hipStream_t s) {
+  const int act = q.act;
+  const bool has_act = act != SMOE_ACT_NONE;
+  char* ws = (char*)q.ws;
+  const size_t dz_bytes = has_act ? ((size_t)q.R * q.N * sizeof(T) + 255) / 256 * 256 : 0;
+  float* part = q.dbias ? (float*)(ws + dz_bytes) : nullptr;
+  const bool need_dz = has_act && (q.dx || q.dw);
+  const int M = act == SMOE_ACT_SWIGLU ? q.N / 2 : q.N;
+  if (need_dz || q.dbias) {
+    const DzArgs d{q.dout, q.z, need_dz ? ws : nullptr, part, q.offsets, q.lddout, q.E, q.R, q.N};
+    const dim3 grid(row_tiles(q.R, q.E, kDzRows), (M + 255) / 256);
+#define SMOE_LD(A) linear_dz_kernel<T, A><<<grid, dim3(256), 0, s>>>(d)
+    SMOE_LIN_ACTS(SMOE_LD);
+#undef SMOE_LD
+  }
+  if (q.dbias)
+    linear_db_kernel<T><<<dim3((q.N + 255) / 256, q.E), dim3(256), 0, s>>>(
+        part, q.offsets, row_tiles(q.R, q.E, kDzRows), q.R, q.N, q.bias_f32, q.dbias);
+  const void* dz = has_act ? (const void*)ws : q.dout;
+  const long long lddz = has_act ? q.N : q.lddout;
+  if (q.dx) {
+    const LinArgs a{dz, q.w, lddz, q.K, nullptr, nullptr, 0, q.offsets, q.dx, nullptr, q.E, q.R, q.N, q.K, 0, 0, 0};
+    linear_any_kernel<T, kDgrad, SMOE_ACT_NONE>
+        <<<dim3(row_tiles(q.R, q.E, kT), (q.K + kT - 1) / kT), dim3(256), 0, s>>>(a);
+  }
+  if (q.dw) {
+    const LinArgs a{dz, q.x, lddz, q.ldx, nullptr, nullptr, 0, q.offsets, q.dw, nullptr, q.E, q.R, q.N, q.K, 0, 0,
+                    q.dw_mode};
+    linear_any_kernel<T, kWgrad, SMOE_ACT_NONE>
+        <<<dim3((q.N + kT - 1) / kT, (q.K + kT - 1) / kT, q.E), dim3(256), 0, s>>>(a);
+  }
+  SMOE_RETURN_LAUNCH();
+}
+
+static int check_linear(int R, int N, int K, int E, int act, int dtype, const int32_t* offsets) {
+  if (R <= 0 || N <= 0 || K <= 0) return SMOE_EINVAL_DIM;
+  if (E <= 0 || E > SMOE_MAX_EXPERTS) return SMOE_EINVAL_EXPERTS;
+  if (act < SMOE_ACT_NONE || act > SMOE_ACT_SWIGLU) return SMOE_EINVAL_MODE;
+  if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_EINVAL_MODE;
+  if (act == SMOE_ACT_SWIGLU && N % 2) return SMOE_EINVAL_DIM;
+  if (E > 1 && !offsets) return SMOE_EINVAL_NULL;
+  if ((uintptr_t)offsets & 3u) return SMOE_EINVAL_PTRALIGN;
+  // what a grid's edges hold
+  if (N > kLinearMaxDim || K > kLinearMaxDim || R > kLinearMaxRows) return SMOE_EINVAL_DIM;
+  return SMOE_OK;
+}
+
+}  // namespace smoe
+
+using namespace smoe;
+
+extern "C" size_t smoe_linear_act_workspace_size(int R, int N, int K, int E, int act) {
+  (void)R, (void)N, (void)K, (void)E, (void)act;
+  return 0;
+}
+
+extern "C" int smoe_linear_act(const smoe_linear_fwd* q, void* stream) {
+  if (!q) return SMOE_EINVAL_NULL;
+  const int st = check_linear(q->R, q->N, q->K, q->E, q->act, q->dtype, q->offsets);
+  if (st) return st;
+  if (q->ldx < 0 || q->ldr < 0) return SMOE_EINVAL_DIM;
+  SMOE_CHECK_ELT(q->x, q->dtype);
+  SMOE_CHECK_ELT(q->w, q->dtype);
+  SMOE_CHECK_ELT(q->out, q->dtype);
+  SMOE_CHECK_OPT(q->bias, q->bias_f32 ? SMOE_F32 : q->dtype);
+  SMOE_CHECK_OPT(q->residual, q->dtype);
+  SMOE_CHECK_OPT(q->z, q->dtype);
+  const LinArgs a{q->x, q->w, q->ldx, q->K, q->bias, q->residual, q->ldr, q->offsets, q->out, q->z,
+                  q->E, q->R, q->N, q->K, q->bias_f32, q->act, 0};
+  hipStream_t s = (hipStream_t)stream;
+  return q->dtype == SMOE_BF16 ? linear_fwd<bf16_t>(a, s) : linear_fwd<f16_t>(a, s);
+}
+
+extern "C" size_t smoe_linear_act_bwd_workspace_size(int R, int N, int K, int E, int act, int with_bias) {
+  (void)K;
+  if (R <= 0 || N <= 0 || E <= 0) return 0;
+  const size_t dz = act != SMOE_ACT_NONE ? ((size_t)R * N * 2 + 255) / 256 * 256 : 0;
+  const size_t part = with_bias ? (size_t)row_tiles(R, E, kDzRows) * N * sizeof(float) : 0;
+  return dz + part;
+}
+
+extern "C" int smoe_linear_act_bwd(const smoe_linear_bwd* q, void* stream) {
+  if (!q) return SMOE_EINVAL_NULL;
+  const int st = check_linear(q->R, q->N, q->K, q->E, q->act, q->dtype, q->offsets);
+  if (st) return st;
+  if (q->lddout < 0 || q->ldx < 0) return SMOE_EINVAL_DIM;
+  if (q->dw_mode < SMOE_WGRAD_F32 || q->dw_mode > SMOE_WGRAD_BF16_ACC) return SMOE_EINVAL_MODE;
+  SMOE_CHECK_ELT(q->dout, q->dtype);
+  if (q->act != SMOE_ACT_NONE) SMOE_CHECK_ELT(q->z, q->dtype);
+  if (q->dx) SMOE_CHECK_ELT(q->w, q->dtype);
+  if (q->dw) SMOE_CHECK_ELT(q->x, q->dtype);
+  SMOE_CHECK_OPT(q->dx, q->dtype);
+  SMOE_CHECK_OPT(q->dw, q->dw_mode < SMOE_WGRAD_BF16 ? SMOE_F32 : q->dtype);
+  SMOE_CHECK_OPT(q->dbias, q->bias_f32 ? SMOE_F32 : q->dtype);
+  const size_t need = smoe_linear_act_bwd_workspace_size(q->R, q->N, q->K, q->E, q->act, q->dbias != nullptr);
+  if (need && (!q->ws || q->ws_bytes < need)) return SMOE_EINVAL_WORKSPACE;
+  if ((uintptr_t)q->ws & 15u) return SMOE_EINVAL_PTRALIGN;
+  hipStream_t s = (hipStream_t)stream;
+  return q->dtype == SMOE_BF16 ? linear_bwd<bf16_t>(*q, s) : linear_bwd<f16_t>(*q, s);
+}

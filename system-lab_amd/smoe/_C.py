@@ -14,6 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsmoe.so")
 
 c_int, c_size_t, c_void_p, c_char_p = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_char_p
+c_float, L = ctypes.c_float, ctypes.c_longlong
 P = c_void_p  # every device pointer travels as an untyped address
 
 # name -> (restype, argtypes); the complete export list of include/smoe.h
@@ -82,6 +83,22 @@ SIGNATURES = {
     "smoe_layer_backward": (c_int, [P, P, P]),
     "smoe_combine_bwd_quant_cols": (c_int, [P, P, P, c_int, c_int, c_int, P, c_int, c_int, P, P,
                                             P, c_int, P]),
+    "smoe_permute_tokens": (c_int, [P, L, P, P, c_int, c_int, c_int, c_int, P, P]),
+    "smoe_permute_tokens_bwd": (c_int, [P, L, P, L, P, P, c_int, c_int, c_int, c_int, P, P, P]),
+    "smoe_unpermute_tokens": (c_int, [P, L, P, P, c_int, c_int, c_int, c_int, P, P]),
+    "smoe_unpermute_tokens_bwd": (c_int, [P, L, P, L, P, P, c_int, c_int, c_int, c_int, P, P, P]),
+    "smoe_block_norm_in": (c_int, [P, L, P, c_int, c_float, c_int, c_int, c_int, P, P, P]),
+    "smoe_block_norm_out": (c_int, [P, L, P, L, P, P, L, c_int, c_int, c_float, c_float, c_int, c_int, c_int,
+                                    P, P, P]),
+    "smoe_block_norm_bwd_workspace_size": (c_size_t, [c_int, c_int]),
+    "smoe_block_norm_in_bwd": (c_int, [P, L, P, L, P, P, c_int, P, L, c_float, c_int, c_int, c_int, P, P, P,
+                                       c_size_t, P]),
+    "smoe_block_norm_out_bwd": (c_int, [P, L, P, L, P, P, P, L, c_int, c_int, c_int, c_int, c_int, P, P, P, P,
+                                        c_size_t, P]),
+    "smoe_linear_act_workspace_size": (c_size_t, [c_int] * 5),
+    "smoe_linear_act": (c_int, [P, P]),
+    "smoe_linear_act_bwd_workspace_size": (c_size_t, [c_int] * 6),
+    "smoe_linear_act_bwd": (c_int, [P, P]),
 }
 
 
@@ -101,6 +118,20 @@ class LayerBwd(ctypes.Structure):
                                     "offsets", "c1", "h", "y", "w1t", "w1ts", "w2t", "w2ts", "dx", "dw1",
                                     "dw2", "dtopk_w", "dlogits", "dyq", "dys", "dh", "dxs", "scratch")]
                 + [("scratch_bytes", c_size_t)])
+
+
+class LinearFwd(ctypes.Structure):
+    """smoe_linear_fwd"""
+    _fields_ = ([(n, c_int) for n in ("R", "N", "K", "E", "act", "dtype", "bias_f32")]
+                + [("x", P), ("ldx", L), ("w", P), ("bias", P), ("residual", P), ("ldr", L), ("offsets", P),
+                   ("out", P), ("z", P), ("ws", P), ("ws_bytes", c_size_t)])
+
+
+class LinearBwd(ctypes.Structure):
+    """smoe_linear_bwd"""
+    _fields_ = ([(n, c_int) for n in ("R", "N", "K", "E", "act", "dtype", "bias_f32", "dw_mode")]
+                + [("dout", P), ("lddout", L), ("x", P), ("ldx", L)]
+                + [(n, P) for n in ("w", "z", "offsets", "dx", "dw", "dbias", "ws")] + [("ws_bytes", c_size_t)])
 
 
 # libsmoe_probe.so: the benchmark's HBM traffic-mix probe, kept out of the
