@@ -116,6 +116,64 @@ __device__ __forceinline__ bool find_row_tile(const int32_t* offsets, int E, int
   return false;
 }
 
+// The same map with the number of tiles known: one pass over the experts by
+// every wave for itself, each lane counting a run of neighbouring experts.
+struct RowTiles {
+  int total;         // row tiles of all experts
+  int first, count;  // of this lane's experts: their first tile, how many
+  __device__ __forceinline__ RowTiles(const int32_t* offsets, int E, int R, int bm) {
+    first = 0;
+    if (!offsets) {
+      total = count = (R + bm - 1) / bm;
+      return;
+    }
+    const int lane = threadIdx.x & 63, per = (E + 63) / 64;
+    int n = 0;
+    for (int i = 0; i < per; ++i) {
+      const int e = lane * per + i;
+      if (e < E) {
+        const int r = clamp_row(offsets, e + 1, R) - clamp_row(offsets, e, R);
+        n += r > 0 ? (r + bm - 1) / bm : 0;
+      }
+    }
+    int inc = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(inc, d, 64);
+      if (lane >= d) inc += up;
+    }
+    count = n;
+    first = inc - n;
+    total = __builtin_amdgcn_readlane(inc, 63);
+  }
+  // Tile `tile` < total; wave-uniform.
+  __device__ __forceinline__ bool find(const int32_t* offsets, int E, int R, int bm, int tile, RowTile* out) const {
+    if (!offsets) {
+      out->e = out->lo = 0;
+      out->row0 = tile * bm;
+      out->rows = R - tile * bm < bm ? R - tile * bm : bm;
+      return out->rows > 0;
+    }
+    const unsigned long long hit = __ballot(tile >= first && tile < first + count);
+    if (!hit) return false;
+    const int src = __builtin_ctzll(hit), per = (E + 63) / 64;
+    int at = tile - __builtin_amdgcn_readlane(first, src);
+    for (int e = src * per; e < E && e < (src + 1) * per; ++e) {
+      const int lo = clamp_row(offsets, e, R), n = clamp_row(offsets, e + 1, R) - lo;
+      const int t = n > 0 ? (n + bm - 1) / bm : 0;
+      if (at < t) {
+        out->e = e;
+        out->lo = lo;
+        out->row0 = lo + at * bm;
+        out->rows = n - at * bm < bm ? n - at * bm : bm;
+        return true;
+      }
+      at -= t;
+    }
+    return false;
+  }
+};
+
 // The forward's and the gradients' common description of one product.
 struct LinArgs {
   const void *a, *b;      // a: rows of the left operand, b: of the right one
@@ -128,5 +186,10 @@ struct LinArgs {
   int E, R, N, K;         // N: rows of the weight, K: its row length
   int bias_f32, act, mode;
 };
+
+// smoe_linear_mm.hip: the tiled kernels, for operands they cover.  what: 0 the
+// product, 1 dx, 2 dW.
+bool linear_mm_ok(const LinArgs& a, int what);
+int linear_mm(const LinArgs& a, int what, int dtype, hipStream_t s);
 
 }  // namespace smoe

@@ -335,6 +335,7 @@ static int row_tiles(int R, int E, int bm) { return (R + bm - 1) / bm + E - 1; }
 
 template <class T>
 static int linear_fwd(const LinArgs& a, hipStream_t s) {
+  if (linear_mm_ok(a, kFwd)) return linear_mm(a, kFwd, Elt<T>::kDtype, s);
   const int act = a.act;
   const int cols = act == SMOE_ACT_SWIGLU ? a.N / 2 : a.N, bn = act == SMOE_ACT_SWIGLU ? kT / 2 : kT;
   const dim3 grid(row_tiles(a.R, a.E, kT), (cols + bn - 1) / bn);
@@ -367,12 +368,18 @@ static int linear_bwd(const smoe_linear_bwd& q, hipStream_t s) {
   const long long lddz = has_act ? q.N : q.lddout;
   if (q.dx) {
     const LinArgs a{dz, q.w, lddz, q.K, nullptr, nullptr, 0, q.offsets, q.dx, nullptr, q.E, q.R, q.N, q.K, 0, 0, 0};
-    linear_any_kernel<T, kDgrad, SMOE_ACT_NONE>
-        <<<dim3(row_tiles(q.R, q.E, kT), (q.K + kT - 1) / kT), dim3(256), 0, s>>>(a);
+    if (linear_mm_ok(a, kDgrad)) {
+      const int st = linear_mm(a, kDgrad, q.dtype, s);
+      if (st) return st;
+    } else {
+      linear_any_kernel<T, kDgrad, SMOE_ACT_NONE>
+          <<<dim3(row_tiles(q.R, q.E, kT), (q.K + kT - 1) / kT), dim3(256), 0, s>>>(a);
+    }
   }
   if (q.dw) {
     const LinArgs a{dz, q.x, lddz, q.ldx, nullptr, nullptr, 0, q.offsets, q.dw, nullptr, q.E, q.R, q.N, q.K, 0, 0,
                     q.dw_mode};
+    if (linear_mm_ok(a, kWgrad)) return linear_mm(a, kWgrad, q.dtype, s);
     linear_any_kernel<T, kWgrad, SMOE_ACT_NONE>
         <<<dim3((q.N + kT - 1) / kT, (q.K + kT - 1) / kT, q.E), dim3(256), 0, s>>>(a);
   }

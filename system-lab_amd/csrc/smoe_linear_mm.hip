@@ -1,0 +1,449 @@
+// smoe_linear_mm.hip — the tiled MFMA kernels of linear_act and its gradients
+// for operands whose rows are 16-byte aligned (gfx950).
+//
+// One kernel, three products (kWhat):
+//   kFwd    D[m][n] = sum_k x[m][k] W[n][k]    both summed along their rows
+//   kDgrad  D[m][k] = sum_n dz[m][n] W[n][k]   W's rows run across the sum
+//   kWgrad  D[n][k] = sum_r dz[r][n] x[r][k]   both operands' rows run across it
+//
+// A workgroup owns a kBM x kBN tile of one expert, a wave kRB x kCB blocks of
+// 16 x 16 of it.  Each step stages 64 terms of the sum of both operands in
+// LDS by direct global->LDS loads, two stages deep: the next step's loads are
+// in flight during this step's MFMAs.
+//
+// "Row" operands (the sum along the row) lie in LDS as 128-byte rows in the
+// swizzled order of smoe_mfma.h and are read 16 bytes a lane.  "Turned"
+// operands lie as they do in memory, 64 rows of the tile's columns, and are
+// read by ds_read_b64_tr_b16, which hands every lane four rows of one column:
+// no transposed copy of weights or activations is ever made.  Their 16-byte
+// chunks are swizzled by the row so that the 16 lanes of a read touch
+// distinct banks.
+//
+// The right operand goes into the MFMA first, so that a lane holds four
+// neighbouring columns of one output row; and the tile's columns are dealt
+// to the blocks such that a lane's kCB blocks are neighbours too: it stores
+// whole 16-byte pieces, with no staging.  For SwiGLU the blocks alternate
+// between gate and up rows of W, and gate and up of a value meet in a lane.
+//
+// Terms past the end of the sum (K % 64, an expert's last rows) are loaded
+// from a 16-byte zero for both operands.  Rows and columns past the tile's end
+// repeat the last valid ones and are not stored.
+#include "smoe_linear.h"
+#include "smoe_mfma.h"
+
+namespace smoe {
+
+__device__ __attribute__((aligned(16))) const uint32_t g_zero16[4] = {0, 0, 0, 0};
+
+enum { kFwd = 0, kDgrad = 1, kWgrad = 2 };
+constexpr int kStep = 64;  // terms of the sum a step: 128 bytes of a row operand
+
+// A direct load of 16 bytes a lane from the lane's own address.
+__device__ __forceinline__ void dma16_at(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+}
+
+typedef short v4s_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s_t* lds_v4s;
+
+template <int kWR_, int kWN_, int kRB_, int kCB_>
+struct MmCfg {
+  static constexpr int kWR = kWR_, kWN = kWN_, kRB = kRB_, kCB = kCB_;
+  static constexpr int kWaves = kWR * kWN, kThreads = kWaves * 64;
+  static constexpr int kBM = kWR * kRB * 16, kBN = kWN * kCB * 16;
+  static constexpr int kABytes = kBM * 128, kBBytes = kBN * 128, kStage = kABytes + kBBytes;
+  static constexpr int kASegs = kABytes / 1024 / kWaves, kBSegs = kBBytes / 1024 / kWaves;
+  static_assert(kASegs * kWaves * 1024 == kABytes && kBSegs * kWaves * 1024 == kBBytes, "segments");
+  static_assert(2 * kStage <= 160 * 1024, "LDS");
+};
+
+// Swizzles of turned operands: XORed into the 16-byte chunk index of row k.
+// Left: a read takes 4 rows x 32 contiguous bytes, so rows move by 32-byte
+// units.  Right: 4 rows x 4 pieces of 8 bytes, one in each of the lane
+// quarters' column runs; the two free bits among the chunk index's low four
+// (one bank round) are bits 0 and 3 for runs of 16 columns, 0 and 1 for 32.
+__device__ __forceinline__ int swz_left(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) << 1; }
+template <int kCB>
+__device__ __forceinline__ int swz_right(int k) {
+  return kCB == 4 ? (k & 1) | ((k >> 1) & 1) << 3 : k & 3;
+}
+
+// Column of the tile (within a wave's kCB * 16) that block j's index r
+// (0..15, four to a lane quarter) stands for.
+template <int kCB>
+__device__ __forceinline__ int col_of(int j, int r) {
+  return (r >> 2) * (kCB * 4) + j * 4 + (r & 3);
+}
+
+template <class T, class C, int kWhat, int kAct>
+__global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs a) {
+  constexpr int kBM = C::kBM, kBN = C::kBN, kRB = C::kRB, kCB = C::kCB;
+  constexpr int kASegs = C::kASegs, kBSegs = C::kBSegs;
+  constexpr bool kPair = kWhat == kFwd && kAct == SMOE_ACT_SWIGLU;
+  constexpr bool kTurnA = kWhat == kWgrad, kTurnB = kWhat != kFwd;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * C::kStage];
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wid / C::kWN, wn = wid % C::kWN;
+
+  // ---- this workgroup's tile --------------------------------------------
+  // cols: columns of the output; kBNo: of them, this tile's
+  const int cols = kWhat == kFwd ? (kPair ? a.N / 2 : a.N) : a.K;
+  constexpr int kBNo = kPair ? kBN / 2 : kBN;
+  const int NT = (cols + kBNo - 1) / kBNo;
+  int e, m0, mrows, n0, len, lo = 0;
+  if constexpr (kWhat == kWgrad) {
+    // tiles of one expert side by side; each XCD takes a contiguous share
+    const int MT = (a.N + kBM - 1) / kBM, total = MT * NT * a.E;
+    const int chunk = (total + 7) / 8, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    const int tile = xcd * chunk + at;
+    if (at >= chunk || tile >= total) return;
+    e = tile / (MT * NT);
+    const int q = tile - e * (MT * NT);
+    m0 = q % MT * kBM;
+    n0 = q / MT * kBNo;
+    mrows = a.N - m0;
+    int hi = a.R;
+    if (a.offsets) {
+      lo = clamp_row(a.offsets, e, a.R);
+      hi = clamp_row(a.offsets, e + 1, a.R);
+    }
+    len = hi > lo ? hi - lo : 0;
+    if (len == 0 && (a.mode & 1)) return;  // nothing to add
+  } else {
+    // row tiles in groups of kGM by all column tiles, rows fastest, so that
+    // an XCD's compute units share 4 row tiles and 8 column tiles at a time
+    constexpr int kGM = 4;
+    const RowTiles rt(a.offsets, a.E, a.R, kBM);
+    const int total = rt.total * NT;
+    const int chunk = (total + 7) / 8, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+    const int tile = xcd * chunk + at;
+    if (at >= chunk || tile >= total) return;
+    const int g = tile / (kGM * NT), q = tile - g * (kGM * NT);
+    const int gm = rt.total - g * kGM < kGM ? rt.total - g * kGM : kGM;
+    RowTile t;
+    if (!rt.find(a.offsets, a.E, a.R, kBM, g * kGM + q % gm, &t)) return;
+    e = t.e;
+    m0 = t.row0;
+    mrows = t.rows;
+    n0 = q / gm * kBNo;
+    len = kWhat == kFwd ? a.K : a.N;
+  }
+  mrows = mrows < kBM ? mrows : kBM;
+  const int ncols = cols - n0 < kBNo ? cols - n0 : kBNo;
+  const int steps = (len + kStep - 1) / kStep;
+  const int full = len / kStep;
+
+  // ---- loaders ------------------------------------------------------------
+  const T* A = (const T*)a.a + (kTurnA ? (long long)lo * a.lda + m0 : (long long)m0 * a.lda);
+  const T* B = (const T*)a.b;
+  if constexpr (kWhat == kFwd) B += (size_t)e * a.N * a.K;
+  else if constexpr (kWhat == kDgrad) B += (size_t)e * a.N * a.K + n0;
+  else B += (long long)lo * a.ldb + n0;
+  const uint32_t pa = (uint32_t)a.lda * 2, pb = (uint32_t)a.ldb * 2;  // row pitches in bytes
+  // per segment: the lane's byte offset from the step's base, and the term of
+  // the sum that its 16 bytes (row operands) or its row (turned) start at
+  uint32_t oa[kASegs], ob[kBSegs];
+  auto row_seg = [&](int seg, int* row, int* chunk) {
+    *row = tile_row(seg * 8 + (lane >> 3));
+    *chunk = (lane & 7) ^ (*row & 7);
+  };
+  auto turn_seg = [&](int seg, int width, int* k, int* slot) {
+    const int p = seg * 64 + lane;
+    *k = p / (width / 8);
+    *slot = p % (width / 8);
+  };
+  auto brow = [&](int row) {  // tile row of a row-wise right operand -> W's row
+    const int w = row / (kCB * 16), j = row % (kCB * 16) / 16, r = row & 15;
+    if constexpr (kPair) {
+      int c = w * (kCB * 8) + (r >> 2) * (kCB * 2) + (j >> 1) * 4 + (r & 3);
+      c = n0 + (c < ncols ? c : ncols - 1);
+      return (j & 1) ? cols + c : c;
+    } else {
+      const int c = w * (kCB * 16) + col_of<kCB>(j, r);
+      return n0 + (c < ncols ? c : ncols - 1);
+    }
+  };
+  auto off_a = [&](int j) -> uint32_t {
+    int x, y;
+    if constexpr (kTurnA) {
+      turn_seg(wid * kASegs + j, kBM, &x, &y);
+      const int c = (y ^ swz_left(x)) * 8;
+      return x * pa + (uint32_t)(c < mrows - 8 ? c : mrows - 8) * 2;
+    } else {
+      row_seg(wid * kASegs + j, &x, &y);
+      return (uint32_t)(x < mrows ? x : mrows - 1) * pa + y * 16;
+    }
+  };
+  auto off_b = [&](int j) -> uint32_t {
+    int x, y;
+    if constexpr (kTurnB) {
+      turn_seg(wid * kBSegs + j, kBN, &x, &y);
+      const int c = (y ^ swz_right<kCB>(x)) * 8;
+      return x * pb + (uint32_t)(c < ncols - 8 ? c : ncols - 8) * 2;
+    } else {
+      row_seg(wid * kBSegs + j, &x, &y);
+      return (uint32_t)brow(x) * pb + y * 16;
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kASegs; ++j) oa[j] = off_a(j);
+#pragma unroll
+  for (int j = 0; j < kBSegs; ++j) ob[j] = off_b(j);
+  const size_t sa = kTurnA ? (size_t)kStep * pa : kStep * 2, sb = kTurnB ? (size_t)kStep * pb : kStep * 2;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
+  const uint32_t a_lds = __builtin_amdgcn_readfirstlane(lds0 + wid * kASegs * 1024);
+  const uint32_t b_lds = __builtin_amdgcn_readfirstlane(lds0 + C::kABytes + wid * kBSegs * 1024);
+  const uint8_t* a_base = uniform_ptr((const uint8_t*)A);
+  const uint8_t* b_base = uniform_ptr((const uint8_t*)B);
+  auto issue = [&](int s) {
+    const uint32_t st = (s & 1) * C::kStage;
+    const uint8_t* ga = a_base + s * sa;
+    const uint8_t* gb = b_base + s * sb;
+    if (s < full) {
+#pragma unroll
+      for (int j = 0; j < kASegs; ++j) dma16(ga, oa[j], a_lds + st + j * 1024);
+#pragma unroll
+      for (int j = 0; j < kBSegs; ++j) dma16(gb, ob[j], b_lds + st + j * 1024);
+    } else {
+      // the last, partial step: terms past the end read as zeros
+      const int left = len - s * kStep;
+      int x, y;
+#pragma unroll
+      for (int j = 0; j < kASegs; ++j) {
+        if constexpr (kTurnA) turn_seg(wid * kASegs + j, kBM, &x, &y);
+        else row_seg(wid * kASegs + j, &y, &x), x *= 8;
+        dma16_at(x < left ? (const void*)(ga + oa[j]) : (const void*)g_zero16, a_lds + st + j * 1024);
+      }
+#pragma unroll
+      for (int j = 0; j < kBSegs; ++j) {
+        if constexpr (kTurnB) turn_seg(wid * kBSegs + j, kBN, &x, &y);
+        else row_seg(wid * kBSegs + j, &y, &x), x *= 8;
+        dma16_at(x < left ? (const void*)(gb + ob[j]) : (const void*)g_zero16, b_lds + st + j * 1024);
+      }
+    }
+  };
+
+  // ---- fragments ----------------------------------------------------------
+  // Lane l supplies row l % 16 of a block at the 8 terms 32 kk + 8 (l / 16) ..
+  const int g = lane >> 4, jr = (lane & 15) >> 2, q4 = lane & 3;
+  const uint32_t ra = swz(wr * kRB * 16 + (lane & 15), g), rb = swz(wn * kCB * 16 + (lane & 15), g);
+  // turned: the lane's row of a read is 32 kk + 8 g + 4 h + jr, whose swizzle
+  // does not depend on kk and h
+  uint32_t ta[kTurnA ? kRB : 1], tb[kTurnB ? kCB / 2 : 1];
+  if constexpr (kTurnA) {
+#pragma unroll
+    for (int i = 0; i < kRB; ++i) {
+      const int chunk = (wr * kRB + i) * 2 + (q4 >> 1);
+      ta[i] = (8 * g + jr) * (kBM * 2) + (chunk ^ swz_left(8 * g + jr)) * 16 + (q4 & 1) * 8;
+    }
+  }
+  if constexpr (kTurnB) {
+#pragma unroll
+    for (int j = 0; j < kCB / 2; ++j) {
+      const int chunk = (wn * kCB * 16 + q4 * (kCB * 4)) / 8 + j;
+      tb[j] = (8 * g + jr) * (kBN * 2) + (chunk ^ swz_right<kCB>(8 * g + jr)) * 16;
+    }
+  }
+  auto tr = [&](uint32_t at) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(smem + at));
+  };
+  auto pair_of = [](v4s_t lo4, v4s_t hi4) {
+    return __builtin_bit_cast(v4u_t, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  auto frag_a = [&](uint32_t st, int kk, int i) -> v4u_t {
+    if constexpr (kTurnA) {
+      const uint32_t at = st + ta[i] + kk * 32 * (kBM * 2);
+      return pair_of(tr(at), tr(at + 4 * (kBM * 2)));
+    } else {
+      return *(const v4u_t*)(smem + st + (ra ^ (kk * 64)) + i * 2048);
+    }
+  };
+  auto frag_b = [&](uint32_t st, int kk, int j) -> v4u_t {
+    if constexpr (kTurnB) {
+      const uint32_t at = st + C::kABytes + tb[j >> 1] + (j & 1) * 8 + kk * 32 * (kBN * 2);
+      return pair_of(tr(at), tr(at + 4 * (kBN * 2)));
+    } else {
+      return *(const v4u_t*)(smem + st + C::kABytes + (rb ^ (kk * 64)) + j * 2048);
+    }
+  };
+
+  v4f_t acc[kRB][kCB];
+#pragma unroll
+  for (int i = 0; i < kRB; ++i)
+#pragma unroll
+    for (int j = 0; j < kCB; ++j) acc[i][j] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  if (steps > 0) issue(0);
+  for (int s = 0; s < steps; ++s) {
+    // this step's loads have landed, and every wave is done reading the other
+    // stage: it may be filled again
+    asm volatile("" ::: "memory");
+    wait_vm_lgkm0<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (s + 1 < steps) issue(s + 1);
+    const uint32_t st = (s & 1) * C::kStage;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      v4u_t fb[kCB];
+#pragma unroll
+      for (int j = 0; j < kCB; ++j) fb[j] = frag_b(st, kk, j);
+      v4u_t fa = frag_a(st, kk, 0);
+#pragma unroll
+      for (int i = 0; i < kRB; ++i) {
+        v4u_t fn = fa;
+        if (i + 1 < kRB) fn = frag_a(st, kk, i + 1);
+#pragma unroll
+        for (int j = 0; j < kCB; ++j) acc[i][j] = mfma32<T>(fb[j], fa, acc[i][j]);
+        fa = fn;
+      }
+    }
+  }
+
+  // ---- epilogue -------------------------------------------------------------
+  // lane: rows wr .. + 16 i + lane % 16, kCB * 4 (SwiGLU kCB * 2) columns in a run
+  constexpr int kRun = kPair ? kCB * 2 : kCB * 4;
+  const int c0 = wn * (kPair ? kCB * 8 : kCB * 16) + g * kRun;
+  const int left = ncols - c0;  // columns of this lane's run that exist
+  if (left <= 0) return;
+  const int n = n0 + c0;
+#pragma unroll
+  for (int p = 0; p < kRun / 8; ++p) {
+    const int np = left - p * 8;
+    if (np <= 0) break;
+    float b0[8], b1[8];
+    if constexpr (kWhat == kFwd) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b0[i] = b1[i] = 0.0f;
+      if (a.bias) {
+        load_param<T>(a.bias, a.bias_f32, (size_t)e * a.N + n + p * 8, np, b0);
+        if constexpr (kPair) load_param<T>(a.bias, a.bias_f32, (size_t)e * a.N + cols + n + p * 8, np, b1);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRB; ++i) {
+      const int m = wr * kRB * 16 + i * 16 + (lane & 15);
+      if (m >= mrows) continue;
+      const size_t row = (size_t)m0 + m;
+      float v[8];
+      if constexpr (kWhat == kFwd) {
+        if constexpr (kPair) {
+          float u[8];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            v[t] = acc[i][(p * 2 + t / 4) * 2][t & 3] + b0[t];
+            u[t] = acc[i][(p * 2 + t / 4) * 2 + 1][t & 3] + b1[t];
+          }
+          if (a.z) {
+            store_f32<T>((T*)a.z + row * a.N + n + p * 8, np, v);
+            store_f32<T>((T*)a.z + row * a.N + cols + n + p * 8, np, u);
+          }
+#pragma unroll
+          for (int t = 0; t < 8; ++t) v[t] = act_value<SMOE_ACT_SILU>(v[t]) * u[t];
+        } else {
+#pragma unroll
+          for (int t = 0; t < 8; ++t) v[t] = acc[i][p * 2 + t / 4][t & 3] + b0[t];
+          if (a.z) store_f32<T>((T*)a.z + row * a.N + n + p * 8, np, v);
+#pragma unroll
+          for (int t = 0; t < 8; ++t) v[t] = act_value<kAct>(v[t]);
+        }
+        if (a.residual) {
+          float r[8];
+          load_f32<T>((const T*)a.residual + (long long)row * a.ldr + n + p * 8, np, r);
+#pragma unroll
+          for (int t = 0; t < 8; ++t) v[t] = v[t] + r[t];
+        }
+        store_f32<T>((T*)a.out + row * cols + n + p * 8, np, v);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[t] = acc[i][p * 2 + t / 4][t & 3];
+        if constexpr (kWhat == kDgrad) {
+          store_f32<T>((T*)a.out + row * cols + n + p * 8, np, v);
+        } else {
+          const size_t at = ((size_t)e * a.N + row) * cols + n + p * 8;
+          if (a.mode < 2) {
+            float* d = (float*)a.out + at;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (np <= 4 * h) break;
+              float w[4];
+              if (a.mode & 1) {
+                load_f32<float>(d + 4 * h, np - 4 * h, w);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) v[4 * h + t] = w[t] + v[4 * h + t];
+              }
+              store_f32<float>(d + 4 * h, np - 4 * h, v + 4 * h);
+            }
+          } else {
+            T* d = (T*)a.out + at;
+            if (a.mode & 1) {
+              float w[8];
+              load_f32<T>(d, np, w);
+#pragma unroll
+              for (int t = 0; t < 8; ++t) v[t] = w[t] + v[t];
+            }
+            store_f32<T>(d, np, v);
+          }
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------- launching ---
+typedef MmCfg<2, 4, 8, 4> MmBig;    // 256 x 256, 8 waves
+typedef MmCfg<2, 2, 4, 4> MmSmall;  // 128 x 128, 4 waves
+
+template <class T, class C, int kWhat>
+static int mm_launch(const LinArgs& a, hipStream_t s) {
+  const int cols = kWhat == kFwd ? (a.act == SMOE_ACT_SWIGLU ? a.N / 2 : a.N) : a.K;
+  const int bn = kWhat == kFwd && a.act == SMOE_ACT_SWIGLU ? C::kBN / 2 : C::kBN;
+  const long long nt = (cols + bn - 1) / bn;
+  const long long mt = kWhat == kWgrad ? (long long)((a.N + C::kBM - 1) / C::kBM) * a.E
+                                       : (a.R + C::kBM - 1) / C::kBM + a.E - 1;
+  const long long blocks = (mt * nt + 7) / 8 * 8;
+  if (blocks * C::kThreads > 0xffffffffLL) return SMOE_EINVAL_DIM;
+  const dim3 grid((unsigned)blocks), block(C::kThreads);
+#define SMOE_MM(A) linear_mm_kernel<T, C, kWhat, A><<<grid, block, 0, s>>>(a)
+  if constexpr (kWhat == kFwd) {
+    switch (a.act) {
+      case SMOE_ACT_NONE: SMOE_MM(SMOE_ACT_NONE); break;
+      case SMOE_ACT_RELU: SMOE_MM(SMOE_ACT_RELU); break;
+      case SMOE_ACT_SILU: SMOE_MM(SMOE_ACT_SILU); break;
+      case SMOE_ACT_GELU: SMOE_MM(SMOE_ACT_GELU); break;
+      case SMOE_ACT_GELU_TANH: SMOE_MM(SMOE_ACT_GELU_TANH); break;
+      default: SMOE_MM(SMOE_ACT_SWIGLU); break;
+    }
+  } else {
+    SMOE_MM(SMOE_ACT_NONE);
+  }
+#undef SMOE_MM
+  SMOE_RETURN_LAUNCH();
+}
+
+// Rows of 16-byte pieces at 16-byte addresses, and 256 of them within the 32
+// bits of a lane's offset.
+static bool mm_rows_ok(const void* p, long long ld, int len) {
+  return ((uintptr_t)p & 15u) == 0 && ld % 8 == 0 && len % 8 == 0 && ld <= (1 << 22);
+}
+
+bool linear_mm_ok(const LinArgs& a, int what) {
+  const int ra = what == kFwd ? a.K : a.N;  // the left operand's row length; the right one's is K
+  return mm_rows_ok(a.a, a.lda, ra) && mm_rows_ok(a.b, a.ldb, a.K) &&
+         // a weight's rows are addressed from its expert's first row
+         (what != kFwd || (long long)a.N * a.K * 2 <= 0xffffffffLL);
+}
+
+template <class T>
+static int linear_mm_t(const LinArgs& a, int what, hipStream_t s) {
+  if (what == kFwd) return mm_launch<T, MmBig, kFwd>(a, s);
+  if (what == kDgrad) return mm_launch<T, MmBig, kDgrad>(a, s);
+  return mm_launch<T, MmBig, kWgrad>(a, s);
+}
+
+int linear_mm(const LinArgs& a, int what, int dtype, hipStream_t s) {
+  return dtype == SMOE_BF16 ? linear_mm_t<bf16_t>(a, what, s) : linear_mm_t<f16_t>(a, what, s);
+}
+
+}  // namespace smoe
