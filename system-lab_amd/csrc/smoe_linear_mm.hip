@@ -51,10 +51,11 @@ struct MmCfg {
   static constexpr int kWR = kWR_, kWN = kWN_, kRB = kRB_, kCB = kCB_;
   static constexpr int kWaves = kWR * kWN, kThreads = kWaves * 64;
   static constexpr int kBM = kWR * kRB * 16, kBN = kWN * kCB * 16;
-  static constexpr int kABytes = kBM * 128, kBBytes = kBN * 128, kStage = kABytes + kBBytes;
+  static constexpr int kABytes = kBM * 128, kBBytes = kBN * 128;
+  static constexpr int kB0 = 3 * kABytes, kLds = kB0 + 2 * kBBytes;  // three left stages, two right ones
   static constexpr int kASegs = kABytes / 1024 / kWaves, kBSegs = kBBytes / 1024 / kWaves;
   static_assert(kASegs * kWaves * 1024 == kABytes && kBSegs * kWaves * 1024 == kBBytes, "segments");
-  static_assert(2 * kStage <= 160 * 1024, "LDS");
+  static_assert(kLds <= 160 * 1024, "LDS");
 };
 
 // Swizzles of turned operands: XORed into the 16-byte chunk index of row k.
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   constexpr int kASegs = C::kASegs, kBSegs = C::kBSegs;
   constexpr bool kPair = kWhat == kFwd && kAct == SMOE_ACT_SWIGLU;
   constexpr bool kTurnA = kWhat == kWgrad, kTurnB = kWhat != kFwd;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * C::kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[C::kLds];
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wid / C::kWN, wn = wid % C::kWN;
@@ -92,16 +93,20 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   constexpr int kBNo = kPair ? kBN / 2 : kBN;
   const int NT = (cols + kBNo - 1) / kBNo;
   int e, m0, mrows, n0, len, lo = 0;
+  // Each XCD takes a contiguous share of the tiles.  Their order is row tiles in
+  // groups of kGM by all column tiles, rows fastest (kWgrad: expert by expert),
+  // so that an XCD's 32 compute units share 4 row tiles and 8 column tiles.
+  constexpr int kGM = 4;
   if constexpr (kWhat == kWgrad) {
-    // tiles of one expert side by side; each XCD takes a contiguous share
     const int MT = (a.N + kBM - 1) / kBM, total = MT * NT * a.E;
     const int chunk = (total + 7) / 8, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
     const int tile = xcd * chunk + at;
     if (at >= chunk || tile >= total) return;
     e = tile / (MT * NT);
-    const int q = tile - e * (MT * NT);
-    m0 = q % MT * kBM;
-    n0 = q / MT * kBNo;
+    const int r = tile - e * (MT * NT), g = r / (kGM * NT), q = r - g * (kGM * NT);
+    const int gm = MT - g * kGM < kGM ? MT - g * kGM : kGM;
+    m0 = (g * kGM + q % gm) * kBM;
+    n0 = q / gm * kBNo;
     mrows = a.N - m0;
     int hi = a.R;
     if (a.offsets) {
@@ -111,9 +116,6 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
     len = hi > lo ? hi - lo : 0;
     if (len == 0 && (a.mode & 1)) return;  // nothing to add
   } else {
-    // row tiles in groups of kGM by all column tiles, rows fastest, so that
-    // an XCD's compute units share 4 row tiles and 8 column tiles at a time
-    constexpr int kGM = 4;
     const RowTiles rt(a.offsets, a.E, a.R, kBM);
     const int total = rt.total * NT;
     const int chunk = (total + 7) / 8, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
@@ -193,34 +195,30 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   const size_t sa = kTurnA ? (size_t)kStep * pa : kStep * 2, sb = kTurnB ? (size_t)kStep * pb : kStep * 2;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
   const uint32_t a_lds = __builtin_amdgcn_readfirstlane(lds0 + wid * kASegs * 1024);
-  const uint32_t b_lds = __builtin_amdgcn_readfirstlane(lds0 + C::kABytes + wid * kBSegs * 1024);
+  const uint32_t b_lds = __builtin_amdgcn_readfirstlane(lds0 + C::kB0 + wid * kBSegs * 1024);
   const uint8_t* a_base = uniform_ptr((const uint8_t*)A);
   const uint8_t* b_base = uniform_ptr((const uint8_t*)B);
-  auto issue = [&](int s) {
-    const uint32_t st = (s & 1) * C::kStage;
-    const uint8_t* ga = a_base + s * sa;
-    const uint8_t* gb = b_base + s * sb;
+  // piece j (1 KiB) of step s into the stage at `stage`
+  auto issue_a = [&](int s, int j, uint32_t stage) {
+    const uint8_t* base = a_base + s * sa;
     if (s < full) {
-#pragma unroll
-      for (int j = 0; j < kASegs; ++j) dma16(ga, oa[j], a_lds + st + j * 1024);
-#pragma unroll
-      for (int j = 0; j < kBSegs; ++j) dma16(gb, ob[j], b_lds + st + j * 1024);
+      dma16(base, oa[j], a_lds + stage + j * 1024);
+    } else {  // the last, partial step: terms past the end read as zeros
+      int term, x;
+      if constexpr (kTurnA) turn_seg(wid * kASegs + j, kBM, &term, &x);
+      else row_seg(wid * kASegs + j, &x, &term), term *= 8;
+      dma16_at(term < len - s * kStep ? (const void*)(base + oa[j]) : (const void*)g_zero16, a_lds + stage + j * 1024);
+    }
+  };
+  auto issue_b = [&](int s, int j, uint32_t stage) {
+    const uint8_t* base = b_base + s * sb;
+    if (s < full) {
+      dma16(base, ob[j], b_lds + stage + j * 1024);
     } else {
-      // the last, partial step: terms past the end read as zeros
-      const int left = len - s * kStep;
-      int x, y;
-#pragma unroll
-      for (int j = 0; j < kASegs; ++j) {
-        if constexpr (kTurnA) turn_seg(wid * kASegs + j, kBM, &x, &y);
-        else row_seg(wid * kASegs + j, &y, &x), x *= 8;
-        dma16_at(x < left ? (const void*)(ga + oa[j]) : (const void*)g_zero16, a_lds + st + j * 1024);
-      }
-#pragma unroll
-      for (int j = 0; j < kBSegs; ++j) {
-        if constexpr (kTurnB) turn_seg(wid * kBSegs + j, kBN, &x, &y);
-        else row_seg(wid * kBSegs + j, &y, &x), x *= 8;
-        dma16_at(x < left ? (const void*)(gb + ob[j]) : (const void*)g_zero16, b_lds + st + j * 1024);
-      }
+      int term, x;
+      if constexpr (kTurnB) turn_seg(wid * kBSegs + j, kBN, &term, &x);
+      else row_seg(wid * kBSegs + j, &x, &term), term *= 8;
+      dma16_at(term < len - s * kStep ? (const void*)(base + ob[j]) : (const void*)g_zero16, b_lds + stage + j * 1024);
     }
   };
 
@@ -261,10 +259,10 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   };
   auto frag_b = [&](uint32_t st, int kk, int j) -> v4u_t {
     if constexpr (kTurnB) {
-      const uint32_t at = st + C::kABytes + tb[j >> 1] + (j & 1) * 8 + kk * 32 * (kBN * 2);
+      const uint32_t at = st + C::kB0 + tb[j >> 1] + (j & 1) * 8 + kk * 32 * (kBN * 2);
       return pair_of(tr(at), tr(at + 4 * (kBN * 2)));
     } else {
-      return *(const v4u_t*)(smem + st + C::kABytes + (rb ^ (kk * 64)) + j * 2048);
+      return *(const v4u_t*)(smem + st + C::kB0 + (rb ^ (kk * 64)) + j * 2048);
     }
   };
 
@@ -274,32 +272,89 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
 #pragma unroll
     for (int j = 0; j < kCB; ++j) acc[i][j] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-  if (steps > 0) issue(0);
-  for (int s = 0; s < steps; ++s) {
-    // this step's loads have landed, and every wave is done reading the other
-    // stage: it may be filled again
+  // Each step is two phases of 32 terms; in a phase a wave reads its fragments
+  // and then runs its kRB x kCB MFMAs, with a barrier after either part.  Of
+  // eight waves the second four are one barrier behind the first: each SIMD
+  // has one wave of either half, and while one reads (and sends for the stages
+  // two steps on) the other keeps the matrix unit busy.  In barrier
+  // intervals, the first half reads phase p in 2p and computes it in 2p + 1,
+  // the second half in 2p + 1 and 2p + 2.
+  //
+  // Step s (phases 2s, 2s + 1): both phases' right fragments are read with
+  // the first phase's left ones, so the right stage is free from interval
+  // 4s + 2, when the first half's second phase refills it for step s + 2.  The
+  // left stages are three: that of step s + 2 was last read in interval 4s - 1.
+  // Step s + 2 is first read in interval 4s + 8, so the first half waits for
+  // its pieces before the barrier of 4s + 7, the end of a second phase's
+  // MFMAs, and the second half before the same barrier, the end of a second
+  // phase's reads.  A load has five to four intervals of 512 cycles to land.
+  constexpr bool kHalves = C::kWaves == 8;
+  const bool second = kHalves && wid >= 4;
+  constexpr int kPieces = kASegs + kBSegs;
+  v4u_t fb[2][kCB], fa[kRB];
+  auto barrier = [] {
     asm volatile("" ::: "memory");
-    wait_vm_lgkm0<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + 1 < steps) issue(s + 1);
-    const uint32_t st = (s & 1) * C::kStage;
+  };
+  // every piece but the last step's has landed (all: that one too)
+  auto landed = [&](bool all) {
+    asm volatile("" ::: "memory");
+    if (all) wait_vm_lgkm0<0>();
+    else wait_vm_lgkm0<kPieces>();
+  };
+  auto send = [&](int s, uint32_t sta, uint32_t stb) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      v4u_t fb[kCB];
+    for (int j = 0; j < kBSegs; ++j) issue_b(s, j, stb);
 #pragma unroll
-      for (int j = 0; j < kCB; ++j) fb[j] = frag_b(st, kk, j);
-      v4u_t fa = frag_a(st, kk, 0);
+    for (int j = 0; j < kASegs; ++j) issue_a(s, j, sta);
+  };
+  auto multiply = [&](int kk) {
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int i = 0; i < kRB; ++i) {
-        v4u_t fn = fa;
-        if (i + 1 < kRB) fn = frag_a(st, kk, i + 1);
+    for (int i = 0; i < kRB; ++i)
 #pragma unroll
-        for (int j = 0; j < kCB; ++j) acc[i][j] = mfma32<T>(fb[j], fa, acc[i][j]);
-        fa = fn;
-      }
-    }
+      for (int j = 0; j < kCB; ++j) acc[i][j] = mfma32<T>(fb[kk][j], fa[i], acc[i][j]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  if (steps > 0) {
+    send(0, 0, 0);
+    if (steps > 1) send(1, C::kABytes, C::kBBytes);
+    landed(steps == 1);
+    barrier();
+    if (second) barrier();
   }
+  uint32_t sta = 0, far = 2 * C::kABytes;  // left stages of this step and of two steps on
+  for (int s = 0; s < steps; ++s) {
+    const uint32_t stb = (s & 1) * C::kBBytes;
+    const bool refill = s + 2 < steps;
+#pragma unroll
+    for (int j = 0; j < kCB; ++j) fb[0][j] = frag_b(stb, 0, j);
+#pragma unroll
+    for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 0, i);
+#pragma unroll
+    for (int j = 0; j < kCB; ++j) fb[1][j] = frag_b(stb, 1, j);
+    __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);  // lgkmcnt(0) alone
+    barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(0);
+    __builtin_amdgcn_sched_barrier(0);
+    barrier();
+#pragma unroll
+    for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 1, i);
+    if (refill) send(s + 2, far, stb);
+    if (second) landed(!refill);
+    else __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);
+    barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!second) landed(!refill);
+    barrier();
+    far = sta;
+    sta = sta == 2 * C::kABytes ? 0 : sta + C::kABytes;
+  }
+  if (kHalves && !second && steps > 0) barrier();
 
   // ---- epilogue -------------------------------------------------------------
   // lane: rows wr .. + 16 i + lane % 16, kCB * 4 (SwiGLU kCB * 2) columns in a run
