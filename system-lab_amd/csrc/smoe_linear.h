@@ -185,11 +185,21 @@ struct LinArgs {
   void *out, *z;
   int E, R, N, K;         // N: rows of the weight, K: its row length
   int bias_f32, act, mode;
+  float* part;            // partial sums of `splits` shares of the sum, or NULL
+  int splits;
 };
+
+// smoe_linear_rows.hip: the product for few rows an expert (0 blocks: others).
+int linear_rows_blocks(int R, int E);
+bool linear_rows_better(int R, int N, int E, int act);
+int linear_rows(const LinArgs& a, int dtype, hipStream_t s);
 
 // smoe_linear_mm.hip: the tiled kernels, for operands they cover.  what: 0 the
 // product, 1 dx, 2 dW.
 bool linear_mm_ok(const LinArgs& a, int what);
+// shares that a dense product's sum is cut into, and the bytes of its partial sums
+int linear_mm_splits(int R, int N, int K, int act, int what);
+size_t linear_mm_part_bytes(int R, int N, int K, int act, int what);
 int linear_mm(const LinArgs& a, int what, int dtype, hipStream_t s);
 
 }  // namespace smoe

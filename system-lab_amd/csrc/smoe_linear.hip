@@ -335,7 +335,10 @@ static int row_tiles(int R, int E, int bm) { return (R + bm - 1) / bm + E - 1; }
 
 template <class T>
 static int linear_fwd(const LinArgs& a, hipStream_t s) {
-  if (linear_mm_ok(a, kFwd)) return linear_mm(a, kFwd, Elt<T>::kDtype, s);
+  const bool tiled = linear_mm_ok(a, kFwd);
+  if (tiled ? linear_rows_better(a.R, a.N, a.E, a.act) : linear_rows_blocks(a.R, a.E) != 0)
+    return linear_rows(a, Elt<T>::kDtype, s);
+  if (tiled) return linear_mm(a, kFwd, Elt<T>::kDtype, s);
   const int act = a.act;
   const int cols = act == SMOE_ACT_SWIGLU ? a.N / 2 : a.N, bn = act == SMOE_ACT_SWIGLU ? kT / 2 : kT;
   const dim3 grid(row_tiles(a.R, a.E, kT), (cols + bn - 1) / bn);
@@ -343,6 +346,15 @@ static int linear_fwd(const LinArgs& a, hipStream_t s) {
   SMOE_LIN_ACTS(SMOE_LF);
 #undef SMOE_LF
   SMOE_RETURN_LAUNCH();
+}
+
+// Parts of the gradients' workspace, each a multiple of 256 bytes.
+static size_t linear_bwd_db_bytes(int R, int N, int E, bool bias) {
+  return bias ? ((size_t)row_tiles(R, E, kDzRows) * N * sizeof(float) + 255) / 256 * 256 : 0;
+}
+static size_t linear_bwd_cut_bytes(int R, int N, int K) {
+  const size_t x = linear_mm_part_bytes(R, N, K, 0, kDgrad), w = linear_mm_part_bytes(R, N, K, 0, kWgrad);
+  return x > w ? x : w;
 }
 
 template <class T>
@@ -364,10 +376,14 @@ static int linear_bwd(const smoe_linear_bwd& q, hipStream_t s) {
   if (q.dbias)
     linear_db_kernel<T><<<dim3((q.N + 255) / 256, q.E), dim3(256), 0, s>>>(
         part, q.offsets, row_tiles(q.R, q.E, kDzRows), q.R, q.N, q.bias_f32, q.dbias);
+  // both gradients' shares of a cut sum: one after the other in the same place
+  float* cut = nullptr;
+  if (!q.offsets && linear_bwd_cut_bytes(q.R, q.N, q.K))
+    cut = (float*)(ws + dz_bytes + linear_bwd_db_bytes(q.R, q.N, q.E, q.dbias != nullptr));
   const void* dz = has_act ? (const void*)ws : q.dout;
   const long long lddz = has_act ? q.N : q.lddout;
   if (q.dx) {
-    const LinArgs a{dz, q.w, lddz, q.K, nullptr, nullptr, 0, q.offsets, q.dx, nullptr, q.E, q.R, q.N, q.K, 0, 0, 0};
+    const LinArgs a{dz, q.w, lddz, q.K, nullptr, nullptr, 0, q.offsets, q.dx, nullptr, q.E, q.R, q.N, q.K, 0, 0, 0, cut, 1};
     if (linear_mm_ok(a, kDgrad)) {
       const int st = linear_mm(a, kDgrad, q.dtype, s);
       if (st) return st;
@@ -378,7 +394,7 @@ static int linear_bwd(const smoe_linear_bwd& q, hipStream_t s) {
   }
   if (q.dw) {
     const LinArgs a{dz, q.x, lddz, q.ldx, nullptr, nullptr, 0, q.offsets, q.dw, nullptr, q.E, q.R, q.N, q.K, 0, 0,
-                    q.dw_mode};
+                    q.dw_mode, cut, 1};
     if (linear_mm_ok(a, kWgrad)) return linear_mm(a, kWgrad, q.dtype, s);
     linear_any_kernel<T, kWgrad, SMOE_ACT_NONE>
         <<<dim3((q.N + kT - 1) / kT, (q.K + kT - 1) / kT, q.E), dim3(256), 0, s>>>(a);
@@ -404,8 +420,8 @@ static int check_linear(int R, int N, int K, int E, int act, int dtype, const in
 using namespace smoe;
 
 extern "C" size_t smoe_linear_act_workspace_size(int R, int N, int K, int E, int act) {
-  (void)R, (void)N, (void)K, (void)E, (void)act;
-  return 0;
+  if (R <= 0 || N <= 0 || K <= 0 || E != 1 || linear_rows_better(R, N, E, act)) return 0;
+  return linear_mm_part_bytes(R, N, K, act, kFwd);
 }
 
 extern "C" int smoe_linear_act(const smoe_linear_fwd* q, void* stream) {
@@ -419,18 +435,19 @@ extern "C" int smoe_linear_act(const smoe_linear_fwd* q, void* stream) {
   SMOE_CHECK_OPT(q->bias, q->bias_f32 ? SMOE_F32 : q->dtype);
   SMOE_CHECK_OPT(q->residual, q->dtype);
   SMOE_CHECK_OPT(q->z, q->dtype);
+  const size_t need = smoe_linear_act_workspace_size(q->R, q->N, q->K, q->E, q->act);
+  if (need && (!q->ws || q->ws_bytes < need)) return SMOE_EINVAL_WORKSPACE;
+  if ((uintptr_t)q->ws & 15u) return SMOE_EINVAL_PTRALIGN;
   const LinArgs a{q->x, q->w, q->ldx, q->K, q->bias, q->residual, q->ldr, q->offsets, q->out, q->z,
-                  q->E, q->R, q->N, q->K, q->bias_f32, q->act, 0};
+                  q->E, q->R, q->N, q->K, q->bias_f32, q->act, 0, need ? (float*)q->ws : nullptr, 1};
   hipStream_t s = (hipStream_t)stream;
   return q->dtype == SMOE_BF16 ? linear_fwd<bf16_t>(a, s) : linear_fwd<f16_t>(a, s);
 }
 
 extern "C" size_t smoe_linear_act_bwd_workspace_size(int R, int N, int K, int E, int act, int with_bias) {
-  (void)K;
-  if (R <= 0 || N <= 0 || E <= 0) return 0;
+  if (R <= 0 || N <= 0 || K <= 0 || E <= 0) return 0;
   const size_t dz = act != SMOE_ACT_NONE ? ((size_t)R * N * 2 + 255) / 256 * 256 : 0;
-  const size_t part = with_bias ? (size_t)row_tiles(R, E, kDzRows) * N * sizeof(float) : 0;
-  return dz + part;
+  return dz + linear_bwd_db_bytes(R, N, E, with_bias != 0) + (E == 1 ? linear_bwd_cut_bytes(R, N, K) : 0);
 }
 
 extern "C" int smoe_linear_act_bwd(const smoe_linear_bwd* q, void* stream) {

@@ -133,6 +133,14 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   }
   mrows = mrows < kBM ? mrows : kBM;
   const int ncols = cols - n0 < kBNo ? cols - n0 : kBNo;
+  // this workgroup's share of the sum, in whole steps
+  int skip = 0;
+  if (a.splits > 1) {
+    const long long all = (len + kStep - 1) / kStep;
+    skip = (int)(all * blockIdx.y / a.splits);
+    const int end = (int)(all * (blockIdx.y + 1) / a.splits) * kStep;
+    len = (len < end ? len : end) - skip * kStep;
+  }
   const int steps = (len + kStep - 1) / kStep;
   const int full = len / kStep;
 
@@ -196,8 +204,8 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
   const uint32_t a_lds = __builtin_amdgcn_readfirstlane(lds0 + wid * kASegs * 1024);
   const uint32_t b_lds = __builtin_amdgcn_readfirstlane(lds0 + C::kB0 + wid * kBSegs * 1024);
-  const uint8_t* a_base = uniform_ptr((const uint8_t*)A);
-  const uint8_t* b_base = uniform_ptr((const uint8_t*)B);
+  const uint8_t* a_base = uniform_ptr((const uint8_t*)A + skip * sa);
+  const uint8_t* b_base = uniform_ptr((const uint8_t*)B + skip * sb);
   // piece j (1 KiB) of step s into the stage at `stage`
   auto issue_a = [&](int s, int j, uint32_t stage) {
     const uint8_t* base = a_base + s * sa;
@@ -363,6 +371,22 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   const int left = ncols - c0;  // columns of this lane's run that exist
   if (left <= 0) return;
   const int n = n0 + c0;
+  if (a.splits > 1) {  // the share's sums as they are; mm_join_kernel does the rest
+    const size_t width = kPair ? a.N : cols;
+    float* part = a.part + (size_t)blockIdx.y * (kWhat == kWgrad ? a.N : a.R) * width;
+#pragma unroll
+    for (int i = 0; i < kRB; ++i) {
+      const int m = wr * kRB * 16 + i * 16 + (lane & 15);
+      if (m >= mrows) continue;
+      float* d = part + (size_t)(m0 + m) * width + n;
+#pragma unroll
+      for (int j = 0; j < kCB; ++j) {
+        const int c = (kPair ? j >> 1 : j) * 4;
+        if (c < left) store_f32<float>(d + c + (kPair && (j & 1) ? cols : 0), left - c, (const float*)&acc[i][j]);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int p = 0; p < kRun / 8; ++p) {
     const int np = left - p * 8;
@@ -446,6 +470,78 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   }
 }
 
+// The shares of a cut sum added in order, and the product's epilogue.  Four
+// columns a thread.
+template <class T, int kWhat, int kAct>
+__global__ __launch_bounds__(256) void mm_join_kernel(const LinArgs a) {
+  constexpr bool kPair = kWhat == kFwd && kAct == SMOE_ACT_SWIGLU;
+  const int rows = kWhat == kWgrad ? a.N : a.R;
+  const int width = kWhat == kFwd ? a.N : a.K, cols = kPair ? a.N / 2 : width;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * 4, np = cols - c;
+  const size_t row = blockIdx.y, size = (size_t)rows * width;
+  if (np <= 0) return;
+  const float* p = a.part + row * width + c;
+  float v[4], u[4], t[4];
+  load_f32<float>(p, np, v);
+  if constexpr (kPair) load_f32<float>(p + cols, np, u);
+  for (int s = 1; s < a.splits; ++s) {
+    load_f32<float>(p + s * size, np, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = v[i] + t[i];
+    if constexpr (kPair) {
+      load_f32<float>(p + s * size + cols, np, t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = u[i] + t[i];
+    }
+  }
+  auto put = [&](T* d, const float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < np) d[i] = Elt<T>::from_f32(f[i]);
+  };
+  if constexpr (kWhat == kFwd) {
+    auto bias = [&](int n) { return a.bias_f32 ? ((const float*)a.bias)[n] : Elt<T>::to_f32(((const T*)a.bias)[n]); };
+    if (a.bias) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < np) {
+          v[i] = v[i] + bias(c + i);
+          if constexpr (kPair) u[i] = u[i] + bias(cols + c + i);
+        }
+      }
+    }
+    if (a.z) {
+      put((T*)a.z + row * width + c, v);
+      if constexpr (kPair) put((T*)a.z + row * width + cols + c, u);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (kPair) v[i] = act_value<SMOE_ACT_SILU>(v[i]) * u[i];
+      else v[i] = act_value<kAct>(v[i]);
+      if (a.residual && i < np) v[i] = v[i] + Elt<T>::to_f32(((const T*)a.residual)[(long long)row * a.ldr + c + i]);
+    }
+    put((T*)a.out + row * cols + c, v);
+  } else if constexpr (kWhat == kDgrad) {
+    put((T*)a.out + row * width + c, v);
+  } else {
+    const size_t at = row * width + c;
+    if (a.mode < 2) {
+      float* d = (float*)a.out + at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < np) d[i] = (a.mode & 1) ? d[i] + v[i] : v[i];
+    } else {
+      T* d = (T*)a.out + at;
+      if (a.mode & 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < np) v[i] = Elt<T>::to_f32(d[i]) + v[i];
+      }
+      put(d, v);
+    }
+  }
+}
+
 // ------------------------------------------------------------- launching ---
 typedef MmCfg<2, 4, 8, 4> MmBig;    // 256 x 256, 8 waves
 typedef MmCfg<2, 2, 4, 4> MmSmall;  // 128 x 128, 4 waves
@@ -459,8 +555,13 @@ static int mm_launch(const LinArgs& a, hipStream_t s) {
                                        : (a.R + C::kBM - 1) / C::kBM + a.E - 1;
   const long long blocks = (mt * nt + 7) / 8 * 8;
   if (blocks * C::kThreads > 0xffffffffLL) return SMOE_EINVAL_DIM;
-  const dim3 grid((unsigned)blocks), block(C::kThreads);
-#define SMOE_MM(A) linear_mm_kernel<T, C, kWhat, A><<<grid, block, 0, s>>>(a)
+  const dim3 grid((unsigned)blocks, a.splits > 1 ? a.splits : 1), block(C::kThreads);
+  const dim3 jgrid((cols + 1023) / 1024, kWhat == kWgrad ? a.N : a.R);
+#define SMOE_MM(A)                                                                     \
+  do {                                                                                 \
+    linear_mm_kernel<T, C, kWhat, A><<<grid, block, 0, s>>>(a);                        \
+    if (a.splits > 1) mm_join_kernel<T, kWhat, A><<<jgrid, dim3(256), 0, s>>>(a);      \
+  } while (0)
   if constexpr (kWhat == kFwd) {
     switch (a.act) {
       case SMOE_ACT_NONE: SMOE_MM(SMOE_ACT_NONE); break;
@@ -490,11 +591,63 @@ bool linear_mm_ok(const LinArgs& a, int what) {
          (what != kFwd || (long long)a.N * a.K * 2 <= 0xffffffffLL);
 }
 
+// Big tiles need rows to fill them and as many tiles as compute units; small
+// ones run two workgroups a unit.  us big / small, K 4096, N 4096, no
+// experts: R 4096 106 / 134, R 2048 93 / 79, R 512 79 / 51; K 2048, N 1536, 128
+// experts: R 65536 528 / 615, R 16384 246 / 230, R 8192 223 / 188; dx of the
+// same: 485 / 623, 237 / 239, 218 / 193.  dW, whose tiles do not depend on the
+// rows: K = N = 4096 242 / 303 at R 8192, 31 / 30 at 512, 20 / 16 at 128.
+static bool mm_big(const LinArgs& a, int what) {
+  const int cols = what == kFwd && a.act == SMOE_ACT_SWIGLU ? a.N / 2 : what == kFwd ? a.N : a.K;
+  const int bn = what == kFwd && a.act == SMOE_ACT_SWIGLU ? 128 : 256;
+  const long long nt = (cols + bn - 1) / bn;
+  if (what == kWgrad) return nt * ((a.N + 255) / 256) * a.E >= 128;
+  const int rows = a.R / a.E;  // an expert's mean
+  return rows >= 192 && nt * ((rows + 255) / 256) * a.E >= 192;
+}
+
+template <class T, class C>
+static int linear_mm_c(const LinArgs& a, int what, hipStream_t s) {
+  if (what == kFwd) return mm_launch<T, C, kFwd>(a, s);
+  if (what == kDgrad) return mm_launch<T, C, kDgrad>(a, s);
+  return mm_launch<T, C, kWgrad>(a, s);
+}
+
+// A dense product of few tiles cuts its sum into shares that fill the chip
+// (with experts there are tiles enough, or too few rows to matter).  The model:
+// a round of small tiles takes about 0.8 us a step with one workgroup a unit and
+// 1.25 with two; the shares' fp32 sums are written and read at 4 TB/s and
+// joined in a launch of their own (4 us).
+int linear_mm_splits(int R, int N, int K, int act, int what) {
+  const bool pair = what == kFwd && act == SMOE_ACT_SWIGLU;
+  const long long rows = what == kWgrad ? N : R, width = what == kFwd ? N : K, len = what == kFwd ? K : what == kDgrad ? N : R;
+  const int bn = pair ? 64 : 128;
+  const long long cols = pair ? N / 2 : width, tiles = (rows + 127) / 128 * ((cols + bn - 1) / bn);
+  const double steps = (double)((len + kStep - 1) / kStep);
+  if (tiles >= 256 || rows > 65535) return 1;
+  int best = 1;
+  double least = steps * 0.8;
+  for (int s = 2; s <= 16 && s * 4 <= steps; s *= 2) {
+    const long long wgs = tiles * s;
+    const double round = wgs <= 256 ? 0.8 : 1.25 * (double)((wgs + 511) / 512);
+    const double t = round * steps / s + 4.0 + (double)s * rows * width * 8.0 / 4e6;
+    if (t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+size_t linear_mm_part_bytes(int R, int N, int K, int act, int what) {
+  const int s = linear_mm_splits(R, N, K, act, what);
+  return s > 1 ? (size_t)s * (what == kWgrad ? N : R) * (what == kFwd ? N : K) * sizeof(float) : 0;
+}
+
 template <class T>
-static int linear_mm_t(const LinArgs& a, int what, hipStream_t s) {
-  if (what == kFwd) return mm_launch<T, MmBig, kFwd>(a, s);
-  if (what == kDgrad) return mm_launch<T, MmBig, kDgrad>(a, s);
-  return mm_launch<T, MmBig, kWgrad>(a, s);
+static int linear_mm_t(LinArgs a, int what, hipStream_t s) {
+  a.splits = a.part && !a.offsets ? linear_mm_splits(a.R, a.N, a.K, a.act, what) : 1;
+  return a.splits == 1 && mm_big(a, what) ? linear_mm_c<T, MmBig>(a, what, s) : linear_mm_c<T, MmSmall>(a, what, s);
 }
 
 int linear_mm(const LinArgs& a, int what, int dtype, hipStream_t s) {

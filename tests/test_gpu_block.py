@@ -359,7 +359,8 @@ def run_linear(dev, R, K, N, act, dtype, offsets=None, bias=None, residual=False
 
 
 DENSE = [(1, 64, 64), (1, 1, 2), (16, 512, 256), (5, 40, 24), (63, 65, 66), (130, 264, 200), (17, 1000, 514),
-         (300, 33, 130), (257, 512, 384), (600, 1096, 776)]
+         (300, 33, 130), (257, 512, 384), (600, 1096, 776), (2, 4160, 136), (29, 1544, 1050),
+         (50, 704, 96), (200, 2048, 264), (70, 1000, 3000), (2050, 136, 72), (34, 4104, 520)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -372,7 +373,7 @@ def test_linear_dense(dev, R, K, N, act, dtype):
 GROUPED = [(40, 64, 64, [0, 0, 13, 13, 40]), (300, 136, 96, [0, 1, 66, 200, 300]), (7, 129, 34, [0, 7]),
            (513, 256, 256, [0, 128, 256, 257, 257, 257, 513]), (64, 48, 32, [0] * 20 + [64]),
            (200, 72, 640, list(range(0, 201, 2))),
-           (1500, 328, 520, [0, 700, 1000, 1001, 1500]), (900, 64, 272, [0] + [90 * (e // 7) for e in range(1, 71)])]
+           (70, 1030, 96, [0, 3, 3, 20, 55, 70]), (1500, 328, 520, [0, 700, 1000, 1001, 1500]), (900, 64, 272, [0] + [90 * (e // 7) for e in range(1, 71)])]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
