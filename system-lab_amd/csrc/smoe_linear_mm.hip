@@ -49,6 +49,7 @@ typedef __attribute__((address_space(3))) v4s_t* lds_v4s;
 template <int kWR_, int kWN_, int kRB_, int kCB_>
 struct MmCfg {
   static constexpr int kWR = kWR_, kWN = kWN_, kRB = kRB_, kCB = kCB_;
+  static_assert(kCB == 4, "col_of");
   static constexpr int kWaves = kWR * kWN, kThreads = kWaves * 64;
   static constexpr int kBM = kWR * kRB * 16, kBN = kWN * kCB * 16;
   static constexpr int kABytes = kBM * 128, kBBytes = kBN * 128;
@@ -60,20 +61,61 @@ struct MmCfg {
 
 // Swizzles of turned operands: XORed into the 16-byte chunk index of row k.
 // Left: a read takes 4 rows x 32 contiguous bytes, so rows move by 32-byte
-// units.  Right: 4 rows x 4 pieces of 8 bytes, one in each of the lane
-// quarters' column runs; the two free bits among the chunk index's low four
-// (one bank round) are bits 0 and 3 for runs of 16 columns, 0 and 1 for 32.
+// units.  Right: 4 rows x 4 neighbouring chunks, 8 bytes of each, so rows
+// move by four chunks: 16 places of the 256-byte bank round.
 __device__ __forceinline__ int swz_left(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) << 1; }
-template <int kCB>
-__device__ __forceinline__ int swz_right(int k) {
-  return kCB == 4 ? (k & 1) | ((k >> 1) & 1) << 3 : k & 3;
-}
+__device__ __forceinline__ int swz_right(int k) { return (k & 3) << 2; }
 
-// Column of the tile (within a wave's kCB * 16) that block j's index r
-// (0..15, four to a lane quarter) stands for.
-template <int kCB>
-__device__ __forceinline__ int col_of(int j, int r) {
-  return (r >> 2) * (kCB * 4) + j * 4 + (r & 3);
+// Column (of a wave's 64) that block j's index r (0..15, four to a lane
+// quarter) stands for: a quarter's two neighbouring blocks make 8 columns in a
+// run, the four quarters' runs 32, so that one store of 16 bytes a lane
+// writes 64 contiguous bytes of 16 rows.
+__device__ __forceinline__ int col_of(int j, int r) { return (j >> 1) * 32 + (r >> 2) * 8 + (j & 1) * 4 + (r & 3); }
+
+// One output tile: rows m0 .. + mrows, columns n0 .. + ncols of expert e, the
+// sum over len terms from `lo` (kWgrad: the expert's first row; cut sums: the
+// share's first step).
+struct MmTile {
+  int e, m0, mrows, n0, ncols, len;
+  long long lo;
+};
+
+// The weight gradients' tiles first .. last of an XCD: eighths of the work, not
+// of the tiles, as an expert's tiles cost its steps and about kOver more for
+// the store.  Every wave for itself; each lane counts neighbouring experts.
+__device__ __forceinline__ void share_work(const LinArgs& a, int tiles, int xcd, int* first, int* last) {
+  constexpr int kOver = 6;
+  auto cost = [&](int e) {
+    const int n = a.offsets ? clamp_row(a.offsets, e + 1, a.R) - clamp_row(a.offsets, e, a.R) : a.R;
+    return (long long)((n > 0 ? (n + kStep - 1) / kStep : 0) + kOver);
+  };
+  const int lane = threadIdx.x & 63, each = (a.E + 63) / 64;
+  long long mine = 0;
+  for (int i = 0; i < each; ++i)
+    if (lane * each + i < a.E) mine += cost(lane * each + i) * tiles;
+  long long inc = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const long long up = __shfl_up(inc, d, 64);
+    if (lane >= d) inc += up;
+  }
+  const long long total = __shfl(inc, 63, 64);
+  // the first tile that starts at or after a point of the work
+  auto tile_from = [&](long long at) {
+    if (at >= total) return a.E * tiles;
+    const int src = __builtin_ctzll(__ballot(at < inc));
+    long long left = at - __shfl(inc - mine, src, 64);
+    int e = src * each;
+    for (; e < a.E; ++e) {
+      const long long c = cost(e) * tiles;
+      if (left < c) break;
+      left -= c;
+    }
+    const long long c = cost(e);
+    return e * tiles + (int)((left + c - 1) / c);
+  };
+  *first = __builtin_amdgcn_readfirstlane(tile_from(total * xcd / 8));
+  *last = __builtin_amdgcn_readfirstlane(tile_from(total * (xcd + 1) / 8));
 }
 
 template <class T, class C, int kWhat, int kAct>
@@ -92,68 +134,58 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   const int cols = kWhat == kFwd ? (kPair ? a.N / 2 : a.N) : a.K;
   constexpr int kBNo = kPair ? kBN / 2 : kBN;
   const int NT = (cols + kBNo - 1) / kBNo;
-  int e, m0, mrows, n0, len, lo = 0;
-  // Each XCD takes a contiguous share of the tiles.  Their order is row tiles in
-  // groups of kGM by all column tiles, rows fastest (kWgrad: expert by expert),
-  // so that an XCD's 32 compute units share 4 row tiles and 8 column tiles.
+  // Each XCD takes a contiguous share of the tiles, its workgroups in turn.  The
+  // order is row tiles in groups of kGM by all column tiles, rows fastest
+  // (kWgrad: expert by expert), so that an XCD's 32 compute units share 4 row
+  // tiles and 8 column tiles at a time.
   constexpr int kGM = 4;
+  const int xcd = blockIdx.x & 7, per = gridDim.x >> 3;
+  int first, last;  // this XCD's tiles
+  const RowTiles rt(kWhat == kWgrad ? nullptr : a.offsets, a.E, a.R, kBM);
+  const int MT = kWhat == kWgrad ? (a.N + kBM - 1) / kBM : rt.total;
   if constexpr (kWhat == kWgrad) {
-    const int MT = (a.N + kBM - 1) / kBM, total = MT * NT * a.E;
-    const int chunk = (total + 7) / 8, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
-    const int tile = xcd * chunk + at;
-    if (at >= chunk || tile >= total) return;
-    e = tile / (MT * NT);
-    const int r = tile - e * (MT * NT), g = r / (kGM * NT), q = r - g * (kGM * NT);
-    const int gm = MT - g * kGM < kGM ? MT - g * kGM : kGM;
-    m0 = (g * kGM + q % gm) * kBM;
-    n0 = q / gm * kBNo;
-    mrows = a.N - m0;
-    int hi = a.R;
-    if (a.offsets) {
-      lo = clamp_row(a.offsets, e, a.R);
-      hi = clamp_row(a.offsets, e + 1, a.R);
-    }
-    len = hi > lo ? hi - lo : 0;
-    if (len == 0 && (a.mode & 1)) return;  // nothing to add
+    share_work(a, MT * NT, xcd, &first, &last);
   } else {
-    const RowTiles rt(a.offsets, a.E, a.R, kBM);
-    const int total = rt.total * NT;
-    const int chunk = (total + 7) / 8, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
-    const int tile = xcd * chunk + at;
-    if (at >= chunk || tile >= total) return;
-    const int g = tile / (kGM * NT), q = tile - g * (kGM * NT);
-    const int gm = rt.total - g * kGM < kGM ? rt.total - g * kGM : kGM;
-    RowTile t;
-    if (!rt.find(a.offsets, a.E, a.R, kBM, g * kGM + q % gm, &t)) return;
-    e = t.e;
-    m0 = t.row0;
-    mrows = t.rows;
-    n0 = q / gm * kBNo;
-    len = kWhat == kFwd ? a.K : a.N;
+    const int total = MT * NT, chunk = (total + 7) / 8;
+    first = xcd * chunk;
+    last = first + chunk < total ? first + chunk : total;
   }
-  mrows = mrows < kBM ? mrows : kBM;
-  const int ncols = cols - n0 < kBNo ? cols - n0 : kBNo;
-  // this workgroup's share of the sum, in whole steps
-  int skip = 0;
-  if (a.splits > 1) {
-    const long long all = (len + kStep - 1) / kStep;
-    skip = (int)(all * blockIdx.y / a.splits);
-    const int end = (int)(all * (blockIdx.y + 1) / a.splits) * kStep;
-    len = (len < end ? len : end) - skip * kStep;
-  }
-  const int steps = (len + kStep - 1) / kStep;
-  const int full = len / kStep;
+  auto locate = [&](int tile, MmTile* t) {
+    if (tile >= last) return false;
+    t->e = kWhat == kWgrad ? tile / (MT * NT) : 0;
+    t->lo = 0;
+    const int r = tile - t->e * (MT * NT), grp = r / (kGM * NT), q = r - grp * (kGM * NT);
+    const int gm = MT - grp * kGM < kGM ? MT - grp * kGM : kGM;
+    const int mt = grp * kGM + q % gm;
+    t->n0 = q / gm * kBNo;
+    t->ncols = cols - t->n0 < kBNo ? cols - t->n0 : kBNo;
+    if constexpr (kWhat == kWgrad) {
+      t->m0 = mt * kBM;
+      t->mrows = a.N - t->m0;
+      int hi = a.R;
+      if (a.offsets) {
+        t->lo = clamp_row(a.offsets, t->e, a.R);
+        hi = clamp_row(a.offsets, t->e + 1, a.R);
+      }
+      t->len = hi > t->lo ? hi - (int)t->lo : 0;
+    } else {
+      RowTile w;
+      if (!rt.find(a.offsets, a.E, a.R, kBM, mt, &w)) return false;
+      t->e = w.e;
+      t->m0 = w.row0;
+      t->mrows = w.rows;
+      t->len = kWhat == kFwd ? a.K : a.N;
+    }
+    t->mrows = t->mrows < kBM ? t->mrows : kBM;
+    return true;
+  };
 
   // ---- loaders ------------------------------------------------------------
-  const T* A = (const T*)a.a + (kTurnA ? (long long)lo * a.lda + m0 : (long long)m0 * a.lda);
-  const T* B = (const T*)a.b;
-  if constexpr (kWhat == kFwd) B += (size_t)e * a.N * a.K;
-  else if constexpr (kWhat == kDgrad) B += (size_t)e * a.N * a.K + n0;
-  else B += (long long)lo * a.ldb + n0;
   const uint32_t pa = (uint32_t)a.lda * 2, pb = (uint32_t)a.ldb * 2;  // row pitches in bytes
-  // per segment: the lane's byte offset from the step's base, and the term of
-  // the sum that its 16 bytes (row operands) or its row (turned) start at
-  uint32_t oa[kASegs], ob[kBSegs];
+  const size_t sa = kTurnA ? (size_t)kStep * pa : kStep * 2, sb = kTurnB ? (size_t)kStep * pb : kStep * 2;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
+  const uint32_t a_lds = __builtin_amdgcn_readfirstlane(lds0 + wid * kASegs * 1024);
+  const uint32_t b_lds = __builtin_amdgcn_readfirstlane(lds0 + C::kB0 + wid * kBSegs * 1024);
   auto row_seg = [&](int seg, int* row, int* chunk) {
     *row = tile_row(seg * 8 + (lane >> 3));
     *chunk = (lane & 7) ^ (*row & 7);
@@ -163,70 +195,83 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
     *k = p / (width / 8);
     *slot = p % (width / 8);
   };
-  auto brow = [&](int row) {  // tile row of a row-wise right operand -> W's row
-    const int w = row / (kCB * 16), j = row % (kCB * 16) / 16, r = row & 15;
-    if constexpr (kPair) {
-      int c = w * (kCB * 8) + (r >> 2) * (kCB * 2) + (j >> 1) * 4 + (r & 3);
-      c = n0 + (c < ncols ? c : ncols - 1);
-      return (j & 1) ? cols + c : c;
-    } else {
-      const int c = w * (kCB * 16) + col_of<kCB>(j, r);
-      return n0 + (c < ncols ? c : ncols - 1);
+  // of the current tile: steps, whole steps, the operands' first bytes and, by
+  // segment, the lane's byte offset from the step's base
+  int steps, full, len;
+  const uint8_t *a_base, *b_base;
+  uint32_t oa[kASegs], ob[kBSegs];
+  auto setup = [&](const MmTile& t) {
+    long long skip = 0;
+    len = t.len;
+    if (a.splits > 1) {  // this workgroup's share of the sum, in whole steps
+      const long long all = (len + kStep - 1) / kStep;
+      skip = all * blockIdx.y / a.splits;
+      const int end = (int)(all * (blockIdx.y + 1) / a.splits) * kStep;
+      len = (len < end ? len : end) - (int)skip * kStep;
     }
-  };
-  auto off_a = [&](int j) -> uint32_t {
-    int x, y;
-    if constexpr (kTurnA) {
-      turn_seg(wid * kASegs + j, kBM, &x, &y);
-      const int c = (y ^ swz_left(x)) * 8;
-      return x * pa + (uint32_t)(c < mrows - 8 ? c : mrows - 8) * 2;
-    } else {
-      row_seg(wid * kASegs + j, &x, &y);
-      return (uint32_t)(x < mrows ? x : mrows - 1) * pa + y * 16;
-    }
-  };
-  auto off_b = [&](int j) -> uint32_t {
-    int x, y;
-    if constexpr (kTurnB) {
-      turn_seg(wid * kBSegs + j, kBN, &x, &y);
-      const int c = (y ^ swz_right<kCB>(x)) * 8;
-      return x * pb + (uint32_t)(c < ncols - 8 ? c : ncols - 8) * 2;
-    } else {
-      row_seg(wid * kBSegs + j, &x, &y);
-      return (uint32_t)brow(x) * pb + y * 16;
-    }
-  };
+    steps = (len + kStep - 1) / kStep;
+    full = len / kStep;
+    const T* A = (const T*)a.a + (kTurnA ? t.lo * a.lda + t.m0 : (long long)t.m0 * a.lda);
+    const T* B = (const T*)a.b;
+    if constexpr (kWhat == kFwd) B += (size_t)t.e * a.N * a.K;
+    else if constexpr (kWhat == kDgrad) B += (size_t)t.e * a.N * a.K + t.n0;
+    else B += t.lo * a.ldb + t.n0;
+    a_base = uniform_ptr((const uint8_t*)A + skip * sa);
+    b_base = uniform_ptr((const uint8_t*)B + skip * sb);
+    // opaque: the lane's share of the addresses is formed here, tile by tile,
+    // instead of being held over the loop
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
 #pragma unroll
-  for (int j = 0; j < kASegs; ++j) oa[j] = off_a(j);
+    for (int j = 0; j < kASegs; ++j) {
+      const int seg = wid * kASegs + j;
+      if constexpr (kTurnA) {
+        const int p = seg * 64 + ln, k = p / (kBM / 8), c = (p % (kBM / 8) ^ swz_left(k)) * 8;
+        oa[j] = k * pa + (uint32_t)(c < t.mrows - 8 ? c : t.mrows - 8) * 2;
+      } else {
+        const int r = tile_row(seg * 8 + (ln >> 3));
+        oa[j] = (uint32_t)(r < t.mrows ? r : t.mrows - 1) * pa + ((ln & 7) ^ (r & 7)) * 16;
+      }
+    }
 #pragma unroll
-  for (int j = 0; j < kBSegs; ++j) ob[j] = off_b(j);
-  const size_t sa = kTurnA ? (size_t)kStep * pa : kStep * 2, sb = kTurnB ? (size_t)kStep * pb : kStep * 2;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
-  const uint32_t a_lds = __builtin_amdgcn_readfirstlane(lds0 + wid * kASegs * 1024);
-  const uint32_t b_lds = __builtin_amdgcn_readfirstlane(lds0 + C::kB0 + wid * kBSegs * 1024);
-  const uint8_t* a_base = uniform_ptr((const uint8_t*)A + skip * sa);
-  const uint8_t* b_base = uniform_ptr((const uint8_t*)B + skip * sb);
-  // piece j (1 KiB) of step s into the stage at `stage`
-  auto issue_a = [&](int s, int j, uint32_t stage) {
-    const uint8_t* base = a_base + s * sa;
+    for (int j = 0; j < kBSegs; ++j) {
+      const int seg = wid * kBSegs + j;
+      if constexpr (kTurnB) {
+        const int p = seg * 64 + ln, k = p / (kBN / 8), c = (p % (kBN / 8) ^ swz_right(k)) * 8;
+        ob[j] = k * pb + (uint32_t)(c < t.ncols - 8 ? c : t.ncols - 8) * 2;
+      } else {
+        const int row = tile_row(seg * 8 + (ln >> 3));
+        const int w = row / (kCB * 16), b = row % (kCB * 16) / 16, r = row & 15;
+        // SwiGLU: gate and up rows of the same 8 columns a quarter, in turn
+        int c = kPair ? w * 32 + (r >> 2) * 8 + (b >> 1) * 4 + (r & 3) : w * 64 + col_of(b, r);
+        c = t.n0 + (c < t.ncols ? c : t.ncols - 1) + (kPair && (b & 1) ? cols : 0);
+        ob[j] = (uint32_t)c * pb + ((ln & 7) ^ (row & 7)) * 16;
+      }
+    }
+  };
+  // this wave's pieces (1 KiB) of step s into the stages at sta and stb
+  auto send = [&](int s, uint32_t sta, uint32_t stb) __attribute__((always_inline)) {
+    const uint8_t *ga = a_base + s * sa, *gb = b_base + s * sb;
     if (s < full) {
-      dma16(base, oa[j], a_lds + stage + j * 1024);
+#pragma unroll
+      for (int j = 0; j < kBSegs; ++j) dma16(gb, ob[j], b_lds + stb + j * 1024);
+#pragma unroll
+      for (int j = 0; j < kASegs; ++j) dma16(ga, oa[j], a_lds + sta + j * 1024);
     } else {  // the last, partial step: terms past the end read as zeros
+      const int left = len - s * kStep;
       int term, x;
-      if constexpr (kTurnA) turn_seg(wid * kASegs + j, kBM, &term, &x);
-      else row_seg(wid * kASegs + j, &x, &term), term *= 8;
-      dma16_at(term < len - s * kStep ? (const void*)(base + oa[j]) : (const void*)g_zero16, a_lds + stage + j * 1024);
-    }
-  };
-  auto issue_b = [&](int s, int j, uint32_t stage) {
-    const uint8_t* base = b_base + s * sb;
-    if (s < full) {
-      dma16(base, ob[j], b_lds + stage + j * 1024);
-    } else {
-      int term, x;
-      if constexpr (kTurnB) turn_seg(wid * kBSegs + j, kBN, &term, &x);
-      else row_seg(wid * kBSegs + j, &x, &term), term *= 8;
-      dma16_at(term < len - s * kStep ? (const void*)(base + ob[j]) : (const void*)g_zero16, b_lds + stage + j * 1024);
+#pragma unroll
+      for (int j = 0; j < kBSegs; ++j) {
+        if constexpr (kTurnB) turn_seg(wid * kBSegs + j, kBN, &term, &x);
+        else row_seg(wid * kBSegs + j, &x, &term), term *= 8;
+        dma16_at(term < left ? (const void*)(gb + ob[j]) : (const void*)g_zero16, b_lds + stb + j * 1024);
+      }
+#pragma unroll
+      for (int j = 0; j < kASegs; ++j) {
+        if constexpr (kTurnA) turn_seg(wid * kASegs + j, kBM, &term, &x);
+        else row_seg(wid * kASegs + j, &x, &term), term *= 8;
+        dma16_at(term < left ? (const void*)(ga + oa[j]) : (const void*)g_zero16, a_lds + sta + j * 1024);
+      }
     }
   };
 
@@ -247,8 +292,8 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   if constexpr (kTurnB) {
 #pragma unroll
     for (int j = 0; j < kCB / 2; ++j) {
-      const int chunk = (wn * kCB * 16 + q4 * (kCB * 4)) / 8 + j;
-      tb[j] = (8 * g + jr) * (kBN * 2) + (chunk ^ swz_right<kCB>(8 * g + jr)) * 16;
+      const int chunk = wn * 8 + j * 4 + q4;
+      tb[j] = (8 * g + jr) * (kBN * 2) + (chunk ^ swz_right(8 * g + jr)) * 16;
     }
   }
   auto tr = [&](uint32_t at) {
@@ -275,10 +320,6 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
   };
 
   v4f_t acc[kRB][kCB];
-#pragma unroll
-  for (int i = 0; i < kRB; ++i)
-#pragma unroll
-    for (int j = 0; j < kCB; ++j) acc[i][j] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
 
   // Each step is two phases of 32 terms; in a phase a wave reads its fragments
   // and then runs its kRB x kCB MFMAs, with a barrier after either part.  Of
@@ -311,12 +352,6 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
     if (all) wait_vm_lgkm0<0>();
     else wait_vm_lgkm0<kPieces>();
   };
-  auto send = [&](int s, uint32_t sta, uint32_t stb) {
-#pragma unroll
-    for (int j = 0; j < kBSegs; ++j) issue_b(s, j, stb);
-#pragma unroll
-    for (int j = 0; j < kASegs; ++j) issue_a(s, j, sta);
-  };
   auto multiply = [&](int kk) {
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -325,148 +360,190 @@ __global__ __launch_bounds__(C::kThreads, 1) void linear_mm_kernel(const LinArgs
       for (int j = 0; j < kCB; ++j) acc[i][j] = mfma32<T>(fb[kk][j], fa[i], acc[i][j]);
     __builtin_amdgcn_s_setprio(0);
   };
-  if (steps > 0) {
-    send(0, 0, 0);
+  // the first two steps of a tile, sent while the tile before is stored
+  auto start = [&] {
+    if (steps > 0) send(0, 0, 0);
     if (steps > 1) send(1, C::kABytes, C::kBBytes);
+  };
+  auto sum = [&] {
+#pragma unroll
+    for (int i = 0; i < kRB; ++i)
+#pragma unroll
+      for (int j = 0; j < kCB; ++j) acc[i][j] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+    if (steps == 0) return;
     landed(steps == 1);
     barrier();
     if (second) barrier();
-  }
-  uint32_t sta = 0, far = 2 * C::kABytes;  // left stages of this step and of two steps on
-  for (int s = 0; s < steps; ++s) {
-    const uint32_t stb = (s & 1) * C::kBBytes;
-    const bool refill = s + 2 < steps;
+    uint32_t sta = 0, far = 2 * C::kABytes;  // left stages of this step and of two steps on
+    for (int s = 0; s < steps; ++s) {
+      const uint32_t stb = (s & 1) * C::kBBytes;
+      const bool refill = s + 2 < steps;
 #pragma unroll
-    for (int j = 0; j < kCB; ++j) fb[0][j] = frag_b(stb, 0, j);
+      for (int j = 0; j < kCB; ++j) fb[0][j] = frag_b(stb, 0, j);
 #pragma unroll
-    for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 0, i);
+      for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 0, i);
 #pragma unroll
-    for (int j = 0; j < kCB; ++j) fb[1][j] = frag_b(stb, 1, j);
-    __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);  // lgkmcnt(0) alone
-    barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(0);
-    __builtin_amdgcn_sched_barrier(0);
-    barrier();
+      for (int j = 0; j < kCB; ++j) fb[1][j] = frag_b(stb, 1, j);
+      __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);  // lgkmcnt(0) alone
+      barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(0);
+      __builtin_amdgcn_sched_barrier(0);
+      barrier();
 #pragma unroll
-    for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 1, i);
-    if (refill) send(s + 2, far, stb);
-    if (second) landed(!refill);
-    else __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);
-    barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(1);
-    __builtin_amdgcn_sched_barrier(0);
-    if (!second) landed(!refill);
-    barrier();
-    far = sta;
-    sta = sta == 2 * C::kABytes ? 0 : sta + C::kABytes;
-  }
-  if (kHalves && !second && steps > 0) barrier();
+      for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 1, i);
+      if (refill) send(s + 2, far, stb);
+      if (second) landed(!refill);
+      else __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);
+      barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (!second) landed(!refill);
+      barrier();
+      far = sta;
+      sta = sta == 2 * C::kABytes ? 0 : sta + C::kABytes;
+    }
+    if (kHalves && !second) barrier();
+  };
 
   // ---- epilogue -------------------------------------------------------------
-  // lane: rows wr .. + 16 i + lane % 16, kCB * 4 (SwiGLU kCB * 2) columns in a run
-  constexpr int kRun = kPair ? kCB * 2 : kCB * 4;
-  const int c0 = wn * (kPair ? kCB * 8 : kCB * 16) + g * kRun;
-  const int left = ncols - c0;  // columns of this lane's run that exist
-  if (left <= 0) return;
-  const int n = n0 + c0;
-  if (a.splits > 1) {  // the share's sums as they are; mm_join_kernel does the rest
-    const size_t width = kPair ? a.N : cols;
-    float* part = a.part + (size_t)blockIdx.y * (kWhat == kWgrad ? a.N : a.R) * width;
+  // A lane holds rows 16 i + lane % 16 of its wave's and kRuns runs of 8
+  // columns, 32 columns apart.
+  constexpr int kRuns = kPair ? 1 : 2;
+  auto store = [&](const MmTile& t) {
+    if (kWhat == kWgrad && t.len == 0 && (a.mode & 1)) return;  // nothing to add
+    const int n0 = t.n0 + wn * (kPair ? 32 : 64) + g * 8;
 #pragma unroll
-    for (int i = 0; i < kRB; ++i) {
-      const int m = wr * kRB * 16 + i * 16 + (lane & 15);
-      if (m >= mrows) continue;
-      float* d = part + (size_t)(m0 + m) * width + n;
+    for (int p = 0; p < kRuns; ++p) {
+      const int n = n0 + p * 32, np = t.n0 + t.ncols - n;  // columns of the run that exist
+      if (np <= 0) break;
+      if (a.splits > 1) {  // the share's sums as they are; mm_join_kernel does the rest
+        const size_t width = kPair ? a.N : cols;
+        float* part = a.part + (size_t)blockIdx.y * (kWhat == kWgrad ? a.N : a.R) * width + n;
 #pragma unroll
-      for (int j = 0; j < kCB; ++j) {
-        const int c = (kPair ? j >> 1 : j) * 4;
-        if (c < left) store_f32<float>(d + c + (kPair && (j & 1) ? cols : 0), left - c, (const float*)&acc[i][j]);
+        for (int i = 0; i < kRB; ++i) {
+          const int m = wr * kRB * 16 + i * 16 + (lane & 15);
+          if (m >= t.mrows) continue;
+          float* d = part + (size_t)(t.m0 + m) * width;
+#pragma unroll
+          for (int j = 0; j < kCB / kRuns; ++j) {
+            const int c = (kPair ? j >> 1 : j) * 4;
+            if (c < np)
+              store_f32<float>(d + c + (kPair && (j & 1) ? cols : 0), np - c, (const float*)&acc[i][p * 2 + j]);
+          }
+        }
+        continue;
       }
-    }
-    return;
-  }
-#pragma unroll
-  for (int p = 0; p < kRun / 8; ++p) {
-    const int np = left - p * 8;
-    if (np <= 0) break;
-    float b0[8], b1[8];
-    if constexpr (kWhat == kFwd) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) b0[i] = b1[i] = 0.0f;
-      if (a.bias) {
-        load_param<T>(a.bias, a.bias_f32, (size_t)e * a.N + n + p * 8, np, b0);
-        if constexpr (kPair) load_param<T>(a.bias, a.bias_f32, (size_t)e * a.N + cols + n + p * 8, np, b1);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kRB; ++i) {
-      const int m = wr * kRB * 16 + i * 16 + (lane & 15);
-      if (m >= mrows) continue;
-      const size_t row = (size_t)m0 + m;
-      float v[8];
+      float b0[8], b1[8];
+      v4u_t res[kRB];
+      const bool whole = kWhat == kFwd && a.residual && np >= 8;
       if constexpr (kWhat == kFwd) {
-        if constexpr (kPair) {
-          float u[8];
 #pragma unroll
-          for (int t = 0; t < 8; ++t) {
-            v[t] = acc[i][(p * 2 + t / 4) * 2][t & 3] + b0[t];
-            u[t] = acc[i][(p * 2 + t / 4) * 2 + 1][t & 3] + b1[t];
-          }
-          if (a.z) {
-            store_f32<T>((T*)a.z + row * a.N + n + p * 8, np, v);
-            store_f32<T>((T*)a.z + row * a.N + cols + n + p * 8, np, u);
-          }
-#pragma unroll
-          for (int t = 0; t < 8; ++t) v[t] = act_value<SMOE_ACT_SILU>(v[t]) * u[t];
-        } else {
-#pragma unroll
-          for (int t = 0; t < 8; ++t) v[t] = acc[i][p * 2 + t / 4][t & 3] + b0[t];
-          if (a.z) store_f32<T>((T*)a.z + row * a.N + n + p * 8, np, v);
-#pragma unroll
-          for (int t = 0; t < 8; ++t) v[t] = act_value<kAct>(v[t]);
+        for (int i = 0; i < 8; ++i) b0[i] = b1[i] = 0.0f;
+        if (a.bias) {
+          load_param<T>(a.bias, a.bias_f32, (size_t)t.e * a.N + n, np, b0);
+          if constexpr (kPair) load_param<T>(a.bias, a.bias_f32, (size_t)t.e * a.N + cols + n, np, b1);
         }
-        if (a.residual) {
-          float r[8];
-          load_f32<T>((const T*)a.residual + (long long)row * a.ldr + n + p * 8, np, r);
+        if (whole) {  // all rows' residuals in flight together
 #pragma unroll
-          for (int t = 0; t < 8; ++t) v[t] = v[t] + r[t];
+          for (int i = 0; i < kRB; ++i) {
+            const int m = wr * kRB * 16 + i * 16 + (lane & 15);
+            res[i] = load_piece<T>((const T*)a.residual +
+                                   (long long)(t.m0 + (m < t.mrows ? m : t.mrows - 1)) * a.ldr + n);
+          }
         }
-        store_f32<T>((T*)a.out + row * cols + n + p * 8, np, v);
-      } else {
+      }
 #pragma unroll
-        for (int t = 0; t < 8; ++t) v[t] = acc[i][p * 2 + t / 4][t & 3];
-        if constexpr (kWhat == kDgrad) {
-          store_f32<T>((T*)a.out + row * cols + n + p * 8, np, v);
-        } else {
-          const size_t at = ((size_t)e * a.N + row) * cols + n + p * 8;
-          if (a.mode < 2) {
-            float* d = (float*)a.out + at;
+      for (int i = 0; i < kRB; ++i) {
+        const int m = wr * kRB * 16 + i * 16 + (lane & 15);
+        if (m >= t.mrows) continue;
+        const size_t row = (size_t)t.m0 + m;
+        float v[8];
+        if constexpr (kWhat == kFwd) {
+          if constexpr (kPair) {
+            float u[8];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (np <= 4 * h) break;
-              float w[4];
-              if (a.mode & 1) {
-                load_f32<float>(d + 4 * h, np - 4 * h, w);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) v[4 * h + t] = w[t] + v[4 * h + t];
-              }
-              store_f32<float>(d + 4 * h, np - 4 * h, v + 4 * h);
+            for (int x = 0; x < 8; ++x) {
+              v[x] = acc[i][x / 4 * 2][x & 3] + b0[x];
+              u[x] = acc[i][x / 4 * 2 + 1][x & 3] + b1[x];
             }
+            if (a.z) {
+              store_f32<T>((T*)a.z + row * a.N + n, np, v);
+              store_f32<T>((T*)a.z + row * a.N + cols + n, np, u);
+            }
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = act_value<SMOE_ACT_SILU>(v[x]) * u[x];
           } else {
-            T* d = (T*)a.out + at;
-            if (a.mode & 1) {
-              float w[8];
-              load_f32<T>(d, np, w);
 #pragma unroll
-              for (int t = 0; t < 8; ++t) v[t] = w[t] + v[t];
+            for (int x = 0; x < 8; ++x) v[x] = acc[i][p * 2 + x / 4][x & 3] + b0[x];
+            if (a.z) store_f32<T>((T*)a.z + row * a.N + n, np, v);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = act_value<kAct>(v[x]);
+          }
+          if (a.residual) {
+            float r[8];
+            if (whole) Elt<T>::unpack(res[i], r);
+            else load_f32<T>((const T*)a.residual + (long long)row * a.ldr + n, np, r);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = v[x] + r[x];
+          }
+          store_f32<T>((T*)a.out + row * cols + n, np, v);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[x] = acc[i][p * 2 + x / 4][x & 3];
+          if constexpr (kWhat == kDgrad) {
+            store_f32<T>((T*)a.out + row * cols + n, np, v);
+          } else {
+            const size_t at = ((size_t)t.e * a.N + row) * cols + n;
+            if (a.mode < 2) {
+              float* d = (float*)a.out + at;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (np <= 4 * h) break;
+                float w[4];
+                if (a.mode & 1) {
+                  load_f32<float>(d + 4 * h, np - 4 * h, w);
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) v[4 * h + x] = w[x] + v[4 * h + x];
+                }
+                store_f32<float>(d + 4 * h, np - 4 * h, v + 4 * h);
+              }
+            } else {
+              T* d = (T*)a.out + at;
+              if (a.mode & 1) {
+                float w[8];
+                load_f32<T>(d, np, w);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] = w[x] + v[x];
+              }
+              store_f32<T>(d, np, v);
             }
-            store_f32<T>(d, np, v);
           }
         }
       }
     }
+  };
+
+  // A workgroup's tiles one after the other: the next one's first two steps are
+  // loaded while this one's results are stored.
+  int tile = first + (blockIdx.x >> 3);
+  MmTile cur;
+  bool have = locate(tile, &cur);
+  if (have) {
+    setup(cur);
+    start();
+  }
+  while (have) {
+    const MmTile done = cur;
+    sum();
+    tile += per;
+    have = locate(tile, &cur);
+    if (have) {
+      setup(cur);
+      start();
+    }
+    store(done);
   }
 }
 
@@ -553,8 +630,10 @@ static int mm_launch(const LinArgs& a, hipStream_t s) {
   const long long nt = (cols + bn - 1) / bn;
   const long long mt = kWhat == kWgrad ? (long long)((a.N + C::kBM - 1) / C::kBM) * a.E
                                        : (a.R + C::kBM - 1) / C::kBM + a.E - 1;
-  const long long blocks = (mt * nt + 7) / 8 * 8;
-  if (blocks * C::kThreads > 0xffffffffLL) return SMOE_EINVAL_DIM;
+  if (mt * nt > 0x7fffffffLL) return SMOE_EINVAL_DIM;
+  // as many workgroups as run at once, each with its share of the tiles
+  constexpr long long kRun = C::kLds > 80 * 1024 ? 256 : 512;
+  const long long blocks = mt * nt < kRun ? (mt * nt + 7) / 8 * 8 : kRun;
   const dim3 grid((unsigned)blocks, a.splits > 1 ? a.splits : 1), block(C::kThreads);
   const dim3 jgrid((cols + 1023) / 1024, kWhat == kWgrad ? a.N : a.R);
 #define SMOE_MM(A)                                                                     \
