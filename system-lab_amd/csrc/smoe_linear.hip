@@ -302,13 +302,18 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* part, const
   const int e = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
   int first = 0, count = (R + kDzRows - 1) / kDzRows;
   if (offsets) {
-    // the blocks of the experts before e (every thread for itself: E is small);
+    // the blocks of the experts before e, a wave's lanes counting 64 at a time;
     // bounds out of order may count more blocks than there are
-    for (int i = 0; i <= e; ++i) {
-      int n = clamp_row(offsets, i + 1, R) - clamp_row(offsets, i, R);
-      count = n > 0 ? (n + kDzRows - 1) / kDzRows : 0;
-      if (i < e) first = first + count < blocks ? first + count : blocks;
-    }
+    auto blocks_of = [&](int i) {
+      const int n = clamp_row(offsets, i + 1, R) - clamp_row(offsets, i, R);
+      return n > 0 ? (n + kDzRows - 1) / kDzRows : 0;
+    };
+    int before = 0;
+    for (int i = threadIdx.x & 63; i < e; i += 64) before += blocks_of(i);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) before += __shfl_xor(before, d, 64);
+    first = before < blocks ? before : blocks;
+    count = blocks_of(e);
     if (count > blocks - first) count = blocks - first;
   }
   if (c >= N) return;

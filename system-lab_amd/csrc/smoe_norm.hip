@@ -9,7 +9,7 @@
 //   dw    = sum over rows of g n,   dgate = (dout n w) summed as it was broadcast
 //
 // Every row is read once: W waves of one workgroup hold it in registers (raw
-// 16-byte pieces, NV a lane) between the sum of squares and the scaling, and
+// 16-byte pieces, kNV a lane) between the sum of squares and the scaling, and
 // the parameter vectors come from the caches.  The sums over a row are fp32,
 // lane by lane and then in a fixed tree.  The sums over rows are fp32 too:
 // each workgroup walks its rows with the columns' sums in registers and
@@ -124,136 +124,210 @@ struct NormBwd {
   int T, H, waves, gate_mode, w_f32, gate_f32;
 };
 
-// One row at a time a workgroup, rows blockIdx.x, + gridDim.x, ...
-template <class T, int kNV>
-__global__ __launch_bounds__(1024) void norm_bwd_kernel(const NormBwd a) {
+// A workgroup takes blockDim / 64 / waves rows at a time, one every so many
+// waves: rows blockIdx.x, + gridDim.x, ... of its places.  A lane keeps g weight
+// and v in fp32 between the row's sum and the result (unpacked twice, fp16 took
+// 1.5 times as long: its conversions are slow).
+template <class T, int kNV, int kThreads, int kGate>
+__global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const NormBwd a) {
+  const int gate_mode = kGate < 0 ? a.gate_mode : kGate;
   constexpr int V = Elt<T>::kVec;
-  __shared__ float red[2][2 * kNormMaxWaves];
+  __shared__ float red[2][kNormMaxWaves];
+  extern __shared__ float cols[];  // [H], where the workgroup has several rows
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c0 = threadIdx.x * V, step = a.waves * 64 * V, H = a.H;
-  float col[kNV][V];
+  const int per = (blockDim.x >> 6) / a.waves, place = wave / a.waves, sub = wave % a.waves;
+  const int c0 = (sub * 64 + lane) * V, step = a.waves * 64 * V, H = a.H;
+  // a lane's columns are the same in every row: weight, times a gate a channel,
+  // stays in registers
+  float col[kNV][V], fac[kNV][V];
 #pragma unroll
-  for (int j = 0; j < kNV; ++j)
+  for (int j = 0; j < kNV; ++j) {
+    const int at = c0 + j * step, left = H - at;
 #pragma unroll
-    for (int i = 0; i < V; ++i) col[j][i] = 0.0f;
+    for (int i = 0; i < V; ++i) {
+      col[j][i] = 0.0f;
+      fac[j][i] = 1.0f;
+    }
+    if (left > 0) {
+      if (a.weight) load_param<T>(a.weight, a.w_f32, at, left, fac[j]);
+      if (gate_mode == SMOE_GATE_CHANNEL) {
+        float gate[V];
+        load_param<T>(a.gate, a.gate_f32, at, left, gate);
+#pragma unroll
+        for (int i = 0; i < V; ++i) fac[j][i] = fac[j][i] * gate[i];
+      }
+    }
+  }
   int turn = 0;
-  for (int t = blockIdx.x; t < a.T; t += gridDim.x, turn ^= 1) {
-    const float rstd = a.rstd[t];
-    float gt = 1.0f;
-    if (a.gate_mode == SMOE_GATE_TOKEN)
-      gt = a.gate_f32 ? ((const float*)a.gate)[(long long)t * a.ldgate]
-                      : Elt<T>::to_f32(((const T*)a.gate)[(long long)t * a.ldgate]);
-    const T* gp = (const T*)a.g + (long long)t * a.ldg;
-    const T* vp = (const T*)a.v + (long long)t * a.ldv;
-    float cc[kNV][V], nn[kNV][V];
-    float dot = 0.0f, dg = 0.0f;
+  for (int t0 = blockIdx.x * per; t0 < a.T; t0 += gridDim.x * per, turn ^= 1) {
+    const int t = t0 + place;
+    const bool live = t < a.T;  // the last rows may leave places empty
+    float dot = 0.0f, rstd = 0.0f, gt = 1.0f;
+    v4u_t pg[kNV], pv[kNV], ps[kNV];
+    float cc[kNV][V], vv[kNV][V];
+    auto full_gate = [&](int at, float* gate) {
+      load_param<T>(a.gate, a.gate_f32, (long long)t * a.ldgate + at, H - at, gate);
+    };
+    if (live) {
+      const T* gp = (const T*)a.g + (long long)t * a.ldg;
+      const T* vp = (const T*)a.v + (long long)t * a.ldv;
 #pragma unroll
-    for (int j = 0; j < kNV; ++j) {
-      const int c = c0 + j * step, n = H - c;
-      if (n > 0) {
-        float w[V], gate[V];
-        load_f32<T>(gp + c, n, cc[j]);
-        load_f32<T>(vp + c, n, nn[j]);
-        if (a.weight) load_param<T>(a.weight, a.w_f32, c, n, w);
-        if (a.gate_mode == SMOE_GATE_CHANNEL) load_param<T>(a.gate, a.gate_f32, c, n, gate);
-        else if (a.gate_mode == SMOE_GATE_FULL) load_param<T>(a.gate, a.gate_f32, (long long)t * a.ldgate + c, n, gate);
-        float full[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float g = cc[j][i];
-          nn[j][i] = nn[j][i] * rstd;
-          const float gn = g * nn[j][i];
-          const float gnw = a.weight ? gn * w[i] : gn;
-          if (a.gate_mode == SMOE_GATE_TOKEN) dg = dg + gnw;
-          if (a.gate_mode == SMOE_GATE_FULL) full[i] = gnw;
-          // the column sums are of g n before a gate a channel, which the
-          // column pass applies to the finished sum
-          if (a.gate_mode == SMOE_GATE_FULL) g = g * gate[i];
-          else g = g * gt;
-          col[j][i] = __builtin_fmaf(g, nn[j][i], col[j][i]);
-          if (a.gate_mode == SMOE_GATE_CHANNEL) g = g * gate[i];
-          cc[j][i] = a.weight ? g * w[i] : g;
-          dot = __builtin_fmaf(cc[j][i], nn[j][i], dot);
+      for (int j = 0; j < kNV; ++j) {
+        const int at = c0 + j * step;
+        if (at + V <= H) {
+          pg[j] = load_piece<T>(gp + at);
+          pv[j] = load_piece<T>(vp + at);
+        } else if (at < H) {
+          float f[V];
+          load_f32<T>(gp + at, H - at, f);
+          pg[j] = Elt<T>::pack(f);
+          load_f32<T>(vp + at, H - at, f);
+          pv[j] = Elt<T>::pack(f);
         }
-        if (a.gate_mode == SMOE_GATE_FULL) {
-          if (a.gate_f32) {
-            float* d = (float*)a.dgate + (size_t)t * H + c;
-            store_f32<float>(d, n < 4 ? n : 4, full);
-            if (V == 8 && n > 4) store_f32<float>(d + 4, n - 4, full + (V == 8 ? 4 : 0));
-          } else {
-            store_f32<T>((T*)a.dgate + (size_t)t * H + c, n, full);
+      }
+      if (a.dskip) {
+        const T* sp = (const T*)a.dskip + (long long)t * a.ldskip;
+#pragma unroll
+        for (int j = 0; j < kNV; ++j) {
+          const int at = c0 + j * step;
+          if (at + V <= H) ps[j] = load_piece<T>(sp + at);
+          else if (at < H) {
+            float f[V];
+            load_f32<T>(sp + at, H - at, f);
+            ps[j] = Elt<T>::pack(f);
+          }
+        }
+      }
+      rstd = a.rstd[t];
+      if (gate_mode == SMOE_GATE_TOKEN)
+        gt = a.gate_f32 ? ((const float*)a.gate)[(long long)t * a.ldgate]
+                        : Elt<T>::to_f32(((const T*)a.gate)[(long long)t * a.ldgate]);
+      const float scale = rstd * gt;
+#pragma unroll
+      for (int j = 0; j < kNV; ++j) {
+        const int at = c0 + j * step, left = H - at;
+        if (left > 0) {
+          // the row's sum is of g v weight (times a gate a channel or a value);
+          // rstd and a gate a token are the row's and come in after it
+          float* g = cc[j];
+          float* v = vv[j];
+          float gate[V], dfull[V];
+          Elt<T>::unpack(pg[j], g);
+          Elt<T>::unpack(pv[j], v);
+          if (gate_mode == SMOE_GATE_FULL) full_gate(at, gate);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float c = g[i] * fac[j][i], gv = g[i] * v[i];
+            if (gate_mode == SMOE_GATE_FULL) {
+              dfull[i] = c * v[i] * rstd;
+              c = c * gate[i];
+              gv = gv * gate[i];
+            }
+            g[i] = c;
+            dot = __builtin_fmaf(c, v[i], dot);
+            // a gate a channel is left out of the columns' sums and applied
+            // to the finished ones
+            col[j][i] = __builtin_fmaf(gv, scale, col[j][i]);
+          }
+          if (gate_mode == SMOE_GATE_FULL) {
+            if (a.gate_f32) {
+              float* d = (float*)a.dgate + (size_t)t * H + at;
+              store_f32<float>(d, left < 4 ? left : 4, dfull);
+              if (V == 8 && left > 4) store_f32<float>(d + 4, left - 4, dfull + (V == 8 ? 4 : 0));
+            } else {
+              store_f32<T>((T*)a.dgate + (size_t)t * H + at, left, dfull);
+            }
           }
         }
       }
     }
-    // both row sums; a row's use of its half of red ends before the half is
-    // written again two rows later, past the next row's barrier
     dot = wave_sum_tree(dot);
-    dg = wave_sum_tree(dg);
     if (a.waves > 1) {
-      if (lane == 0) {
-        red[turn][wave] = dot;
-        red[turn][kNormMaxWaves + wave] = dg;
-      }
+      // a row's use of its half of red ends before the half is written again
+      // two rows later, past the next row's barrier
+      if (lane == 0) red[turn][wave] = dot;
       __syncthreads();
       dot = 0.0f;
-      dg = 0.0f;
-      for (int i = 0; i < a.waves; ++i) {
-        dot = dot + red[turn][i];
-        dg = dg + red[turn][kNormMaxWaves + i];
-      }
+      for (int i = 0; i < a.waves; ++i) dot = dot + red[turn][place * a.waves + i];
     }
-    if (a.gate_mode == SMOE_GATE_TOKEN && threadIdx.x == 0) {
-      if (a.gate_f32) ((float*)a.dgate)[t] = dg;
-      else ((T*)a.dgate)[t] = Elt<T>::from_f32(dg);
+    if (!live) continue;
+    dot = dot * rstd;  // sum of g n weight: a token's dgate
+    if (gate_mode == SMOE_GATE_TOKEN && sub == 0 && lane == 0) {
+      if (a.gate_f32) ((float*)a.dgate)[t] = dot;
+      else ((T*)a.dgate)[t] = Elt<T>::from_f32(dot);
     }
-    const float mean = dot / (float)H;
+    // rstd (c - n mean(c n)) = (rstd gate) g weight - (rstd^2 mean(c n)) v
+    const float up = rstd * gt, down = rstd * (rstd * (gt * dot / (float)H));
 #pragma unroll
     for (int j = 0; j < kNV; ++j) {
-      const int c = c0 + j * step, n = H - c;
-      if (n > 0) {
-        float sk[V];
-        if (a.dskip) load_f32<T>((const T*)a.dskip + (long long)t * a.ldskip + c, n, sk);
+      const int at = c0 + j * step, left = H - at;
+      if (left > 0) {
+        float g[V], sk[V];
+        if (a.dskip) Elt<T>::unpack(ps[j], sk);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          float d = rstd * __builtin_fmaf(-nn[j][i], mean, cc[j][i]);
-          if (a.dskip) d = __builtin_fmaf(a.scale, sk[i], d);
-          cc[j][i] = d;
+          float c = __builtin_fmaf(-down, vv[j][i], up * cc[j][i]);
+          if (a.dskip) c = __builtin_fmaf(a.scale, sk[i], c);
+          g[i] = c;
         }
-        store_f32<T>((T*)a.dv + (size_t)t * H + c, n, cc[j]);
+        store_f32<T>((T*)a.dv + (size_t)t * H + at, left, g);
       }
     }
   }
-  if (a.part) {
+  if (!a.part) return;
+  // the places' column sums, added in order, are the workgroup's partial row
+  for (int p = 0; p < per; ++p) {
+    if (p == place) {
 #pragma unroll
-    for (int j = 0; j < kNV; ++j) {
-      const int c = c0 + j * step, n = H - c;
-      if (n > 0) {
-        float* d = a.part + (size_t)blockIdx.x * H + c;
-        store_f32<float>(d, n < 4 ? n : 4, col[j]);
-        if (V == 8 && n > 4) store_f32<float>(d + 4, n - 4, col[j] + (V == 8 ? 4 : 0));
+      for (int j = 0; j < kNV; ++j) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int c = c0 + j * step + i;
+          if (c < H) {
+            if (p > 0) col[j][i] = cols[c] + col[j][i];
+            if (p + 1 < per) cols[c] = col[j][i];
+          }
+        }
+        const int at = c0 + j * step, left = H - at;
+        if (p + 1 == per && left > 0) {
+          float* d = a.part + (size_t)blockIdx.x * H + at;
+          store_f32<float>(d, left < 4 ? left : 4, col[j]);
+          if (V == 8 && left > 4) store_f32<float>(d + 4, left - 4, col[j] + (V == 8 ? 4 : 0));
+        }
       }
     }
+    if (p + 1 < per) __syncthreads();
   }
 }
 
 // The partial rows' column sums S: dweight = S (times a gate a channel), and
-// that gate's gradient S w.  64 columns a workgroup, 4 waves over the rows.
+// that gate's gradient S w.  64 columns a workgroup, 16 waves over the rows.
 template <class T>
-__global__ __launch_bounds__(256) void norm_cols_kernel(const float* part, int G, int H, const void* weight,
-                                                        int w_f32, const void* gate, int gate_f32, void* dweight,
-                                                        void* dgate) {
-  __shared__ float acc[4][64];
+__global__ __launch_bounds__(1024) void norm_cols_kernel(const float* part, int G, int H, const void* weight,
+                                                         int w_f32, const void* gate, int gate_f32, void* dweight,
+                                                         void* dgate) {
+  __shared__ float acc[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int c = blockIdx.x * 64 + lane;
   float s = 0.0f;
-  if (c < H)
-    for (int g = wave; g < G; g += 4) s = s + part[(size_t)g * H + c];
+  if (c < H) {
+    int g = wave;
+    for (; g + 7 * 16 < G; g += 8 * 16) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = part[(size_t)(g + i * 16) * H + c];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = s + v[i];
+    }
+    for (; g < G; g += 16) s = s + part[(size_t)g * H + c];
+  }
   acc[wave][lane] = s;
   __syncthreads();
   if (wave || c >= H) return;
-  s = acc[0][lane] + acc[1][lane] + acc[2][lane] + acc[3][lane];
+  s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s = s + acc[i][lane];
   auto param = [&](const void* p, int f32) { return f32 ? ((const float*)p)[c] : Elt<T>::to_f32(((const T*)p)[c]); };
   auto put = [&](void* p, int f32, float v) {
     if (f32) ((float*)p)[c] = v;
@@ -263,20 +337,30 @@ __global__ __launch_bounds__(256) void norm_cols_kernel(const float* part, int G
   if (dgate) put(dgate, gate_f32, weight ? s * param(weight, w_f32) : s);
 }
 
-// Waves a row (a power of two up to 16) so that a lane holds about two
-// pieces; kNV, the pieces a lane, then covers the rest.
-static int norm_waves(int H, int vec) {
+// Waves a row (a power of two up to 16) so that a lane holds about `pieces`;
+// kNV, the pieces a lane, then covers the rest.
+static int norm_waves(int H, int vec, int pieces) {
   int w = 1;
-  while (w < kNormMaxWaves && 64 * vec * 2 * w < H) w *= 2;
+  while (w < kNormMaxWaves && 64 * vec * pieces * w < H) w *= 2;
   return w;
 }
 
-// Workgroups of the backward pass: enough rows each (8) that the partial
-// rows stay a small part of the traffic, and no more groups than keep the
-// chip full.
-static int norm_bwd_groups(int T) {
-  const int g = (T + 7) / 8;
-  return g < 1024 ? g : 1024;
+// The backward pass: up to six pieces a lane, so that rows up to 3 K 16-bit
+// values need one wave and no barrier; threads of a workgroup, rows it holds at a
+// time; and workgroups: two rows a place at least, so that the partial
+// rows stay a small part of the traffic, two a compute unit at most.
+constexpr int kBwdPieces = 4;
+struct NormBwdPlan {
+  int waves, threads, per, groups;
+};
+static NormBwdPlan norm_bwd_plan(int T, int H, int dtype) {
+  NormBwdPlan p;
+  p.waves = norm_waves(H, dtype == SMOE_F32 ? 4 : 8, kBwdPieces);
+  p.threads = p.waves <= 4 ? 256 : p.waves * 64;
+  p.per = p.threads / 64 / p.waves;
+  const int g = (T + 2 * p.per - 1) / (2 * p.per);
+  p.groups = g < 512 ? g : 512;
+  return p;
 }
 
 static int check_norm(int T, int H, int dtype, int gate_mode, int param_f32) {
@@ -300,7 +384,7 @@ static int check_norm(int T, int H, int dtype, int gate_mode, int param_f32) {
 template <class T, bool kOut>
 static int norm_fwd_launch(NormFwd a, hipStream_t s) {
   constexpr int V = Elt<T>::kVec;
-  a.waves = norm_waves(a.H, V);
+  a.waves = norm_waves(a.H, V, 2);
   const int need = (a.H + a.waves * 64 * V - 1) / (a.waves * 64 * V);
   const int threads = a.waves <= 4 ? 256 : a.waves * 64, per = threads / 64 / a.waves;
   const dim3 grid((a.T + per - 1) / per), block(threads);
@@ -322,15 +406,38 @@ static int norm_fwd_call(const NormFwd& a, int dtype, void* stream) {
 template <class T>
 static int norm_bwd_launch(NormBwd a, void* dweight, void* dgate_ch, hipStream_t s) {
   constexpr int V = Elt<T>::kVec;
-  a.waves = norm_waves(a.H, V);
-  const int need = (a.H + a.waves * 64 * V - 1) / (a.waves * 64 * V);
-  const int G = norm_bwd_groups(a.T);
-  const dim3 grid(G), block(a.waves * 64);
-#define SMOE_NB(NV) norm_bwd_kernel<T, NV><<<grid, block, 0, s>>>(a)
-  SMOE_NORM_NV(need, SMOE_NB);
+  const NormBwdPlan p = norm_bwd_plan(a.T, a.H, Elt<T>::kDtype);
+  a.waves = p.waves;
+  const int need = (a.H + a.waves * 64 * V - 1) / (a.waves * 64 * V), G = p.groups;
+  const dim3 grid(G), block(p.threads);
+  const size_t lds = a.part && p.per > 1 ? a.H * sizeof(float) : 0;
+  if (p.threads <= 256) {
+    // the common row lengths: every count of pieces and every gate by itself
+#define SMOE_NB(NV, GATE) norm_bwd_kernel<T, NV, 256, GATE><<<grid, block, lds, s>>>(a)
+#define SMOE_NBG(NV)                                                   \
+  do {                                                                 \
+    if (a.gate_mode == SMOE_GATE_NONE) SMOE_NB(NV, SMOE_GATE_NONE);    \
+    else if (a.gate_mode == SMOE_GATE_CHANNEL) SMOE_NB(NV, SMOE_GATE_CHANNEL); \
+    else if (a.gate_mode == SMOE_GATE_TOKEN) SMOE_NB(NV, SMOE_GATE_TOKEN);     \
+    else SMOE_NB(NV, SMOE_GATE_FULL);                                  \
+  } while (0)
+    if (need <= 1) SMOE_NBG(1);
+    else if (need <= 2) SMOE_NBG(2);
+    else if (need <= 3) SMOE_NBG(3);
+    else if (need <= 4) SMOE_NBG(4);
+    else SMOE_NBG(6);
+  } else if (p.threads <= 512) {
+    if (need <= 4) norm_bwd_kernel<T, 4, 512, -1><<<grid, block, lds, s>>>(a);
+    else norm_bwd_kernel<T, 6, 512, -1><<<grid, block, lds, s>>>(a);
+  } else {
+    if (need <= 4) norm_bwd_kernel<T, 4, 1024, -1><<<grid, block, lds, s>>>(a);
+    else if (need <= 8) norm_bwd_kernel<T, 8, 1024, -1><<<grid, block, lds, s>>>(a);
+    else norm_bwd_kernel<T, 16, 1024, -1><<<grid, block, lds, s>>>(a);
+  }
+#undef SMOE_NBG
 #undef SMOE_NB
   if (a.part)
-    norm_cols_kernel<T><<<dim3((a.H + 63) / 64), dim3(256), 0, s>>>(
+    norm_cols_kernel<T><<<dim3((a.H + 63) / 64), dim3(1024), 0, s>>>(
         a.part, G, a.H, a.weight, a.w_f32, a.gate_mode == SMOE_GATE_CHANNEL ? a.gate : nullptr, a.gate_f32,
         dweight, dgate_ch);
   SMOE_RETURN_LAUNCH();
@@ -388,7 +495,9 @@ extern "C" int smoe_block_norm_out(const void* y, long long ldy, const void* x, 
 
 extern "C" size_t smoe_block_norm_bwd_workspace_size(int T, int H) {
   if (T <= 0 || H <= 0 || H > kNormMaxH) return 0;
-  return (size_t)norm_bwd_groups(T) * H * sizeof(float);
+  // whichever element type needs more
+  const int a = norm_bwd_plan(T, H, SMOE_BF16).groups, b = norm_bwd_plan(T, H, SMOE_F32).groups;
+  return (size_t)(a > b ? a : b) * H * sizeof(float);
 }
 
 extern "C" int smoe_block_norm_in_bwd(const void* dh, long long lddh, const void* x, long long ldx,
