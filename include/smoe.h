@@ -734,6 +734,12 @@ int smoe_layer_backward(const smoe_layer_bwd* args, void* stream, void* side_str
  */
 int smoe_permute_tokens(const void* x, long long ldx, const int32_t* inv_map, const float* w,
                         int T, int K, int H, int dtype, void* xp, void* stream);
+/* smoe_route_sort of topk_idx [T,K] and permute_tokens by its inv_map, in one
+ * launch up to 2048 pairs; ws as for smoe_route_sort. */
+int smoe_sort_permute_tokens(const void* x, long long ldx, const int32_t* topk_idx, const float* w,
+                             int T, int K, int E, int H, int dtype, int32_t* row_map,
+                             int32_t* inv_map, int32_t* counts, int32_t* offsets, void* xp,
+                             void* ws, size_t ws_bytes, void* stream);
 int smoe_permute_tokens_bwd(const void* dxp, long long lddxp, const void* x, long long ldx,
                             const int32_t* inv_map, const float* w, int T, int K, int H, int dtype,
                             void* dx, float* dw, void* stream);

@@ -120,6 +120,107 @@ __global__ __launch_bounds__(1024) void tokens_kernel(const TokArgs a) {
   }
 }
 
+// The expert sort and the permute of a small batch in one launch.  Every
+// workgroup has all the pairs' expert ids in LDS and finds its tokens' rows
+// by counting: the row of pair p is the number of pairs of a lower expert, and
+// of the same expert before p.  The last workgroup counts the experts' rows.
+// The same bytes as the sort's own launches, which a batch this small would
+// spend more time on than on its rows.
+constexpr int kSortPairs = 2048;
+struct SortArgs {
+  const int32_t* ids;
+  int32_t *row_map, *inv_map, *counts, *offsets, *status;
+  int E;
+};
+template <class T, int kMaxK>
+__global__ __launch_bounds__(1024) void tokens_sort_kernel(const TokArgs a, const SortArgs q) {
+  constexpr int V = Elt<T>::kVec;
+  __shared__ int ids[kSortPairs];
+  __shared__ int hist[SMOE_MAX_EXPERTS], bad;
+  const int K = a.K, H = a.H, R = a.T * K, E = q.E;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool counting = blockIdx.x == gridDim.x - 1;
+  for (int p = threadIdx.x; p < R; p += blockDim.x) ids[p] = q.ids[p];
+  if (counting) {
+    for (int e = threadIdx.x; e < E; e += blockDim.x) hist[e] = 0;
+    if (threadIdx.x == 0) bad = 0;
+  }
+  __syncthreads();
+  if (counting) {
+    for (int p = threadIdx.x; p < R; p += blockDim.x) {
+      const unsigned e = (unsigned)ids[p];
+      if (e < (unsigned)E) atomicAdd(&hist[e], 1);  // whole numbers: any order
+      else atomicAdd(&bad, 1);
+    }
+    __syncthreads();
+    if (wave) return;
+    const int each = (E + 63) / 64;  // a lane's run of neighbouring experts
+    int n = 0;
+    for (int i = 0; i < each; ++i)
+      if (lane * each + i < E) n += hist[lane * each + i];
+    int inc = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(inc, d, 64);
+      if (lane >= d) inc += up;
+    }
+    int at = inc - n;
+    for (int i = 0; i < each; ++i) {
+      const int e = lane * each + i;
+      if (e < E) {
+        q.counts[e] = hist[e];
+        q.offsets[e] = at;
+        at += hist[e];
+        if (e == E - 1) q.offsets[E] = at;
+      }
+    }
+    if (lane == 0) *q.status = bad;
+    return;
+  }
+  const int per = (blockDim.x >> 6) / a.waves, sub = wave % a.waves;
+  const int t = blockIdx.x * per + wave / a.waves;
+  if (t >= a.T) return;
+  int r[kMaxK];
+  float wk[kMaxK];
+#pragma unroll
+  for (int k = 0; k < kMaxK; ++k) {
+    r[k] = -1;
+    wk[k] = 1.0f;
+    if (k < K) {
+      const int p = t * K + k, e = ids[p];
+      if (a.w) wk[k] = a.w[p];
+      if ((unsigned)e < (unsigned)E) {
+        int n = 0;
+        for (int o = lane; o < R; o += 64) {
+          const int f = ids[o];
+          n += (f >= 0 && f < e) || (f == e && o < p);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d, 64);
+        r[k] = __builtin_amdgcn_readfirstlane(n);
+      }
+      if (sub == 0 && lane == 0) {
+        q.inv_map[p] = r[k];
+        if (r[k] >= 0) q.row_map[r[k]] = p;
+      }
+    }
+  }
+  const T* tok = (const T*)a.tok + (long long)t * a.ld_tok;
+  for (int c = (sub * 64 + lane) * V; c < H; c += a.waves * 64 * V) {
+    float x[V], o[V];
+    load_f32<T>(tok + c, H - c, x);
+#pragma unroll
+    for (int k = 0; k < kMaxK; ++k) {
+      if (r[k] >= 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = wk[k] * x[i];
+        store_f32<T>((T*)a.out + (size_t)r[k] * H + c, H - c, o);
+      }
+    }
+  }
+}
+
 // Waves a token: a power of two that makes about 4096 of them (16 a compute
 // unit), but no more than the row has pieces for, and at most 16.
 static int token_waves(int T, int H, int vec) {
@@ -155,6 +256,23 @@ static int tokens_call(const TokArgs& a, int dtype, void* stream) {
   return tokens_launch<float, kScatter, kDot>(a, s);
 }
 
+template <class T>
+static int tokens_sort_launch(TokArgs a, const SortArgs& q, hipStream_t s) {
+  a.waves = token_waves(a.T, a.H, Elt<T>::kVec);
+  const int threads = a.waves <= 4 ? 256 : a.waves * 64;
+  const int per = threads / 64 / a.waves;
+  const dim3 grid((a.T + per - 1) / per + 1), block(threads);
+#define SMOE_TS(MK) tokens_sort_kernel<T, MK><<<grid, block, 0, s>>>(a, q)
+  if (a.K <= 1) SMOE_TS(1);
+  else if (a.K <= 2) SMOE_TS(2);
+  else if (a.K <= 4) SMOE_TS(4);
+  else if (a.K <= 8) SMOE_TS(8);
+  else if (a.K <= 16) SMOE_TS(16);
+  else SMOE_TS(32);
+#undef SMOE_TS
+  SMOE_RETURN_LAUNCH();
+}
+
 static int check_tokens(const int32_t* inv_map, const float* w, int T, int K, int H, int dtype) {
   if (T <= 0 || H <= 0) return SMOE_EINVAL_DIM;
   if (K <= 0 || K > 32) return SMOE_EINVAL_TOPK;
@@ -177,6 +295,35 @@ extern "C" int smoe_permute_tokens(const void* x, long long ldx, const int32_t* 
   SMOE_CHECK_ELT(x, dtype);
   SMOE_CHECK_ELT(xp, dtype);
   return tokens_call<true, false>({x, nullptr, xp, ldx, 0, inv_map, w, nullptr, T, K, H, 1}, dtype, stream);
+}
+
+extern "C" int smoe_sort_permute_tokens(const void* x, long long ldx, const int32_t* topk_idx, const float* w,
+                                        int T, int K, int E, int H, int dtype, int32_t* row_map,
+                                        int32_t* inv_map, int32_t* counts, int32_t* offsets, void* xp, void* ws,
+                                        size_t ws_bytes, void* stream) {
+  int st = check_tokens(inv_map, w, T, K, H, dtype);
+  if (st) return st;
+  if (ldx < 0) return SMOE_EINVAL_DIM;
+  SMOE_CHECK_ELT(x, dtype);
+  SMOE_CHECK_ELT(xp, dtype);
+  if ((long long)T * K > kSortPairs) {
+    st = smoe_route_sort(topk_idx, T, K, E, row_map, inv_map, counts, offsets, ws, ws_bytes, stream);
+    return st ? st : smoe_permute_tokens(x, ldx, inv_map, w, T, K, H, dtype, xp, stream);
+  }
+  if (E <= 0 || E > SMOE_MAX_EXPERTS) return SMOE_EINVAL_EXPERTS;
+  if (K > E) return SMOE_EINVAL_TOPK;
+  if (!topk_idx || !row_map || !counts || !offsets) return SMOE_EINVAL_NULL;
+  if (((uintptr_t)topk_idx | (uintptr_t)row_map | (uintptr_t)counts | (uintptr_t)offsets) & 3u)
+    return SMOE_EINVAL_PTRALIGN;
+  if (!ws || ws_bytes < smoe_route_sort_workspace_size(T, K, E)) return SMOE_EINVAL_WORKSPACE;
+  if ((uintptr_t)ws & 15u) return SMOE_EINVAL_PTRALIGN;
+  const TokArgs a{x, nullptr, xp, ldx, 0, inv_map, w, nullptr, T, K, H, 1};
+  const SortArgs q{topk_idx, row_map, inv_map, counts, offsets,
+                   (int32_t*)((char*)ws + SMOE_ROUTE_STATUS_OFFSET), E};
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == SMOE_BF16) return tokens_sort_launch<bf16_t>(a, q, s);
+  if (dtype == SMOE_F16) return tokens_sort_launch<f16_t>(a, q, s);
+  return tokens_sort_launch<float>(a, q, s);
 }
 
 extern "C" int smoe_permute_tokens_bwd(const void* dxp, long long lddxp, const void* x, long long ldx,

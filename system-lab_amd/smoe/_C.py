@@ -84,6 +84,8 @@ SIGNATURES = {
     "smoe_combine_bwd_quant_cols": (c_int, [P, P, P, c_int, c_int, c_int, P, c_int, c_int, P, P,
                                             P, c_int, P]),
     "smoe_permute_tokens": (c_int, [P, L, P, P, c_int, c_int, c_int, c_int, P, P]),
+    "smoe_sort_permute_tokens": (c_int, [P, L, P, P, c_int, c_int, c_int, c_int, c_int, P, P, P, P, P, P, c_size_t,
+                                         P]),
     "smoe_permute_tokens_bwd": (c_int, [P, L, P, L, P, P, c_int, c_int, c_int, c_int, P, P, P]),
     "smoe_unpermute_tokens": (c_int, [P, L, P, P, c_int, c_int, c_int, c_int, P, P]),
     "smoe_unpermute_tokens_bwd": (c_int, [P, L, P, L, P, P, c_int, c_int, c_int, c_int, P, P, P]),

@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _C
-from .ops import _check, _ptr, _sort_workspace, _stream, route_sort
+from .ops import _check, _ptr, _status_workspace, route_sort
 
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # SMOE_BF16 / _F16 / _F32
 _ALL, _HALF = tuple(DTYPES), (torch.bfloat16, torch.float16)
@@ -24,36 +24,58 @@ NORM_MAX_H = 65536
 _F32 = torch.float32
 
 
-def _rows(t: torch.Tensor, name: str, dtypes, cols: int | None = None, rows: int | None = None) -> int:
-    """Check a 2-D input whose rows may lie apart; -> elements between rows."""
+def _here(t, name: str) -> None:
+    """A tensor on the current GPU (a call's checks cost a few microseconds, as
+    much as a small kernel: cheap questions first)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor (got {t.device}); the HIP kernels are the only path")
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"{name} is on {t.device} but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _stream() -> int:
+    """The current stream's handle on the current device."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _dense(t, name: str, dtypes, shape) -> None:
+    """Check a contiguous tensor of a given shape."""
+    _here(t, name)
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected one of {tuple(dtypes)}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _rows(t: torch.Tensor, name: str, dtypes, cols: int | None = None, rows: int | None = None) -> int:
+    """Check a 2-D input whose rows may lie apart; -> elements between rows."""
+    _here(t, name)
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has dtype {t.dtype}, expected one of {tuple(dtypes)}")
     if t.dim() != 2:
         raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
-    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+    r, c = t.shape
+    if (rows is not None and r != rows) or (cols is not None and c != cols):
         raise ValueError(f"{name} must be [{'*' if rows is None else rows}, {'*' if cols is None else cols}], "
-                         f"got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+                         f"got {(r, c)}")
+    ld, one = t.stride()
+    if one != 1 and c > 1:
         raise ValueError(f"{name}'s rows must be contiguous (strides {t.stride()})")
-    return t.stride(0)
+    return ld
 
 
 def _like(t: torch.Tensor, dtype, shape) -> torch.Tensor:
-    return torch.empty(shape, dtype=dtype, device=t.device)
+    return t.new_empty(shape, dtype=dtype)
 
 
 def _out(out: torch.Tensor | None, like: torch.Tensor, shape, name: str = "out") -> torch.Tensor:
     if out is None:
         return _like(like, like.dtype, shape)
-    _check(out, name, (like.dtype,))
-    if tuple(out.shape) != tuple(shape):
-        raise ValueError(f"{name} must be {list(shape)}, got {list(out.shape)}")
+    _dense(out, name, (like.dtype,), shape)
     return out
 
 
@@ -65,9 +87,7 @@ def _pairs(inv_map, top_k: int, topk_w, T: int) -> None:
     if inv_map.numel() != T * top_k:
         raise ValueError(f"inv_map must have T*K = {T * top_k} entries, got {inv_map.numel()}")
     if topk_w is not None:
-        _check(topk_w, "topk_w", (_F32,), 2)
-        if tuple(topk_w.shape) != (T, top_k):
-            raise ValueError(f"topk_w must be [{T}, {top_k}], got {list(topk_w.shape)}")
+        _dense(topk_w, "topk_w", (_F32,), (T, top_k))
 
 
 def _tokens_of(rows: int, top_k: int, name: str) -> int:
@@ -98,16 +118,28 @@ def permute_tokens(x: torch.Tensor, topk_idx: torch.Tensor, num_experts: int, to
     router's weights applied on the way in where ``topk_w`` [T,K] is given.
     x [T,H], topk_idx [T,K] i32 -> (xp [T*K,H], row_map, inv_map, counts,
     offsets) as ``route_sort`` numbers the rows."""
-    _rows(x, "x", _ALL)
-    _check(topk_idx, "topk_idx", (torch.int32,), 2)
-    if topk_idx.shape[0] != x.shape[0]:
-        raise ValueError("topk_idx must have T rows")
-    if x.shape[0] == 0:
-        i32 = dict(dtype=torch.int32, device=x.device)
-        return (_like(x, x.dtype, (0, x.shape[1])), torch.empty(0, **i32), torch.empty(0, **i32),
-                torch.zeros(num_experts, **i32), torch.zeros(num_experts + 1, **i32))
-    row_map, inv_map, counts, offsets = route_sort(topk_idx, num_experts)
-    return permute_tokens_rows(x, inv_map, topk_idx.shape[1], topk_w), row_map, inv_map, counts, offsets
+    ld = _rows(x, "x", _ALL)
+    T, H = x.shape
+    _here(topk_idx, "topk_idx")
+    if topk_idx.dim() != 2 or topk_idx.shape[0] != T:
+        raise ValueError(f"topk_idx must be [{T}, K], got {list(topk_idx.shape)}")
+    K, E, i32 = topk_idx.shape[1], int(num_experts), torch.int32
+    _dense(topk_idx, "topk_idx", (i32,), (T, K))
+    if not 0 < K <= min(E, 32):
+        raise ValueError(f"top-k must be in [1, min(E, 32)], got {K} of {E}")
+    if topk_w is not None:
+        _dense(topk_w, "topk_w", (_F32,), (T, K))
+    R = T * K
+    xp, row_map, inv_map = x.new_empty((R, H)), x.new_empty(R, dtype=i32), x.new_empty(R, dtype=i32)
+    counts, offsets = x.new_empty(E, dtype=i32), x.new_empty(E + 1, dtype=i32)
+    if T == 0:
+        return xp, row_map, inv_map, counts.zero_(), offsets.zero_()
+    if H == 0:
+        return (xp, *route_sort(topk_idx, E))
+    ws = _status_workspace(int(_C.lib().smoe_route_sort_workspace_size(T, K, E)), x.device)
+    _C.call("smoe_sort_permute_tokens", _ptr(x), ld, _ptr(topk_idx), _ptr(topk_w), T, K, E, H, DTYPES[x.dtype],
+            _ptr(row_map), _ptr(inv_map), _ptr(counts), _ptr(offsets), _ptr(xp), _ptr(ws), ws.numel(), _stream())
+    return xp, row_map, inv_map, counts, offsets
 
 
 def unpermute_tokens(y: torch.Tensor, inv_map: torch.Tensor, top_k: int, topk_w: torch.Tensor | None = None,
@@ -165,18 +197,12 @@ def unpermute_tokens_bwd(dout: torch.Tensor, inv_map: torch.Tensor, top_k: int, 
 
 
 # ------------------------------------------------------------------- norms
-def _norm_param(p, name: str, like: torch.Tensor) -> None:
-    _check(p, name, (like.dtype, _F32))
-
-
 def _norm_weight(weight, v: torch.Tensor) -> int:
     if not 0 < v.shape[1] <= NORM_MAX_H:
         raise ValueError(f"rows must have 1 to {NORM_MAX_H} values, got {v.shape[1]}")
     if weight is None:
         return 0
-    _norm_param(weight, "weight", v)
-    if tuple(weight.shape) != (v.shape[1],):
-        raise ValueError(f"weight must be [{v.shape[1]}], got {list(weight.shape)}")
+    _dense(weight, "weight", (v.dtype, _F32), (v.shape[1],))
     return int(weight.dtype == _F32)
 
 
@@ -187,9 +213,7 @@ def _norm_gate(gate, v: torch.Tensor):
     T, H = v.shape
     f32 = int(gate.dtype == _F32)
     if gate.dim() == 1:
-        _norm_param(gate, "gate", v)
-        if gate.shape[0] != H:
-            raise ValueError(f"a gate a channel must be [{H}], got {list(gate.shape)}")
+        _dense(gate, "gate", (v.dtype, _F32), (H,))
         return 1, 0, f32
     ld = _rows(gate, "gate", (v.dtype, _F32), None, T)
     if gate.shape[1] == 1 and H != 1:
@@ -206,9 +230,7 @@ def _eps(eps: float) -> float:
 
 
 def _rstd(rstd, T: int) -> None:
-    _check(rstd, "rstd", (_F32,), 1)
-    if rstd.numel() != T:
-        raise ValueError(f"rstd must be [{T}], got {list(rstd.shape)}")
+    _dense(rstd, "rstd", (_F32,), (T,))
 
 
 def block_norm_in(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6):
@@ -298,7 +320,10 @@ def _linear_weight(w, x: torch.Tensor, act: str, bias, offsets):
     """(E, N, K) of a weight [N,K], or [E,N,K] with offsets [E+1]."""
     if act not in ACTS:
         raise ValueError(f"act must be one of {sorted(ACTS)}, got {act!r}")
-    _check(w, "w", (x.dtype,), 2 if offsets is None else 3)
+    _here(w, "w")
+    if w.dim() != (2 if offsets is None else 3):
+        raise ValueError(f"w must be [N, K], or [E, N, K] with offsets; got shape {tuple(w.shape)}")
+    _dense(w, "w", (x.dtype,), w.shape)
     E = 1 if offsets is None else w.shape[0]
     N, K = w.shape[-2:]
     if x.shape[1] != K:
@@ -306,13 +331,9 @@ def _linear_weight(w, x: torch.Tensor, act: str, bias, offsets):
     if act == "swiglu" and N % 2:
         raise ValueError("w's rows must be gate | up halves for act='swiglu'")
     if offsets is not None:
-        _check(offsets, "offsets", (torch.int32,), 1)
-        if offsets.numel() != E + 1:
-            raise ValueError("offsets must have E+1 entries")
+        _dense(offsets, "offsets", (torch.int32,), (E + 1,))
     if bias is not None:
-        _check(bias, "bias", (x.dtype, _F32))
-        if tuple(bias.shape) != tuple(w.shape[:-1]):
-            raise ValueError(f"bias must be {list(w.shape[:-1])}, got {list(bias.shape)}")
+        _dense(bias, "bias", (x.dtype, _F32), w.shape[:-1])
     if not (E and N and K):
         raise ValueError(f"w must not be empty, got {list(w.shape)}")
     return E, N, K
@@ -366,15 +387,11 @@ def linear_act_bwd(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, z: torc
     if act != "none":
         if z is None:
             raise ValueError(f"the gradient of act={act!r} needs z (linear_act's save_z)")
-        _check(z, "z", (x.dtype,), 2)
-        if tuple(z.shape) != (R, N):
-            raise ValueError(f"z must be [{R}, {N}], got {list(z.shape)}")
+        _dense(z, "z", (x.dtype,), (R, N))
     if accumulate and dw_out is None:
         raise ValueError("accumulate needs the buffer to add into (dw_out)")
     if dw_out is not None:
-        _check(dw_out, "dw_out", (_F32, w.dtype))
-        if dw_out.shape != w.shape:
-            raise ValueError(f"dw_out must be {list(w.shape)}, got {list(dw_out.shape)}")
+        _dense(dw_out, "dw_out", (_F32, w.dtype), w.shape)
     dx = _like(x, x.dtype, (R, K)) if need_dx else None
     dw = (dw_out if dw_out is not None else torch.empty_like(w)) if need_dw else None
     db = None if bias is None else torch.empty_like(bias)

@@ -25,6 +25,12 @@ def test_tokens_reject():
     assert p(x=MIS) == -6 and p(xp=MIS) == -6 and p(inv=FAKE + 2) == -6 and p(w=FAKE + 2) == -6
     assert p(x=FAKE + 2, dt=2) == -6
     assert p(T=1 << 30, K=1, H=1) == -2  # more workgroups than a grid holds
+    need = lib.smoe_route_sort_workspace_size(4, 2, 8)
+    q = lambda idx=FAKE, T=4, K=2, E=8, rm=FAKE, xp=FAKE, ws=FAKE, nb=need, ld=64: lib.smoe_sort_permute_tokens(
+        FAKE, ld, idx, None, T, K, E, 64, 0, rm, FAKE, FAKE, FAKE, xp, ws, nb, None)
+    assert q(idx=None) == -1 and q(rm=None) == -1 and q(xp=None) == -1 and q(ws=None) == -5 and q(nb=need - 1) == -5
+    assert q(E=0) == -4 and q(E=1025) == -4 and q(E=1) == -7 and q(T=0) == -2 and q(ld=-1) == -2 and q(ws=FAKE + 8) == -6
+    assert q(T=2000, idx=None, nb=1 << 30) == -1 and q(T=2000, nb=4) == -5
     b = lambda g=FAKE, x=FAKE, dx=FAKE, dw=FAKE, T=4: lib.smoe_permute_tokens_bwd(
         g, 64, x, 64, FAKE, FAKE, T, 2, 64, 0, dx, dw, None)
     assert b(g=None) == -1 and b(x=None) == -1 and b(dx=None) == -1 and b(T=-1) == -2 and b(dw=FAKE + 2) == -6

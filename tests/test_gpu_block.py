@@ -119,6 +119,23 @@ def test_unpermute_and_gradients(dev, T, H, K, E, weights, dtype):
         check(dw, prod.sum(2), (H + 1) * E32 * prod.abs().sum(2), "dw of unpermute")
 
 
+@pytest.mark.parametrize("T,E,K", [(1, 8, 8), (256, 1024, 8), (1024, 3, 2), (1025, 3, 2), (64, 1000, 32), (2048, 5, 1)])
+def test_permute_sort_against_route_sort(dev, T, E, K):
+    """Maps, counts, offsets and the status of a small batch in one launch
+    and of a larger one are the sort's, repeated and out-of-range ids among
+    them."""
+    g = torch.Generator().manual_seed(T)
+    idx = torch.randint(-2, E + 2, (T, K), generator=g, dtype=torch.int32).to(dev)
+    x = rand((T, 24), F16, 1).to(dev)
+    got = smoe.permute_tokens(x, idx, E)
+    status = int(smoe.last_route_status(dev))
+    want = smoe.route_sort(idx, E)
+    n = int(want[3][-1])
+    assert status == int(smoe.last_route_status(dev)) == T * K - n
+    assert got[1][:n].equal(want[0][:n]) and all(a.equal(b) for a, b in zip(got[2:], want[1:]))
+    assert got[0][:n].equal(x[(want[0][:n] // K).long()])
+
+
 def test_tokens_rows_apart_and_odd_starts(dev):
     """Inputs whose rows lie apart or start at an odd element, and one row
     repeated (stride 0), give what contiguous copies give."""
