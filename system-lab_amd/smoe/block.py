@@ -63,7 +63,7 @@ def _rows(t: torch.Tensor, name: str, dtypes, cols: int | None = None, rows: int
         raise ValueError(f"{name} must be [{'*' if rows is None else rows}, {'*' if cols is None else cols}], "
                          f"got {(r, c)}")
     ld, one = t.stride()
-    if one != 1 and c > 1:
+    if one != 1 and c > 1 and r > 0:
         raise ValueError(f"{name}'s rows must be contiguous (strides {t.stride()})")
     return ld
 

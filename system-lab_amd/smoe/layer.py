@@ -14,7 +14,7 @@ import ctypes
 import torch
 from torch import nn
 
-from . import _C, ops
+from . import _C, block, ops
 
 
 # Optimizer steps seen in this process.  Megatron-style optimizers write the
@@ -102,6 +102,72 @@ class _GateLinear(torch.autograd.Function):
         return dx, dw, None
 
 
+def _rows_grad(g: torch.Tensor) -> torch.Tensor:
+    """A gradient as the operators take it: autograd may hand over an expanded
+    one, or one of other strides."""
+    return g if g.shape[-1] <= 1 or g.stride(-1) == 1 else g.contiguous()
+
+
+class _BlockNormIn(torch.autograd.Function):
+    """(h, x): the norm before the block, and x on to the residual, so that the
+    backward adds the residual's gradient in the norm's own pass.  What comes
+    back for x is the gradient of the block's output, still without the
+    residual's scale (_BlockNormOut)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, eps, scale):
+        h, rstd = block.block_norm_in(x, weight, eps)
+        ctx.save_for_backward(x, weight, rstd)
+        ctx.scale = scale
+        return h, x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, dh, dskip):
+        x, weight, rstd = ctx.saved_tensors
+        dx, dw = block.block_norm_in_bwd(_rows_grad(dh), x, rstd, weight,
+                                         dskip=None if dskip is None else _rows_grad(dskip), skip_scale=ctx.scale)
+        return dx, dw, None, None
+
+
+class _BlockNormOut(torch.autograd.Function):
+    """residual_scale * x + gate * norm(y); the gradient it returns for x is
+    dout itself, which _BlockNormIn scales."""
+
+    @staticmethod
+    def forward(ctx, y, x, weight, gate, scale, eps):
+        out, rstd = block.block_norm_out(y, x, weight, gate=gate, residual_scale=scale, eps=eps)
+        ctx.save_for_backward(y, weight, gate, rstd)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        y, weight, gate, rstd = ctx.saved_tensors
+        dout = _rows_grad(dout)
+        dy, dw, dg = block.block_norm_out_bwd(dout, y, rstd, weight, gate=gate)
+        return dy, dout, dw, dg, None, None
+
+
+class _LinearAct(torch.autograd.Function):
+    """act(x W^T) + residual with its gradients; a weight with a ``main_grad``
+    has its gradient added into that, as the experts' weights have."""
+
+    @staticmethod
+    def forward(ctx, x, w, act, residual):
+        out, z = block.linear_act(x, w, act=act, residual=residual, save_z=True) if act != "none" else (
+            block.linear_act(x, w, residual=residual), None)
+        ctx.save_for_backward(x, w, z)
+        ctx.act, ctx.main_grad = act, getattr(w, "main_grad", None)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        x, w, z = ctx.saved_tensors
+        dout, need, mg = _rows_grad(dout), ctx.needs_input_grad, ctx.main_grad
+        dx, dw, _ = block.linear_act_bwd(dout, x, w, z=z, act=ctx.act, need_dx=need[0], need_dw=need[1],
+                                         dw_out=mg, accumulate=mg is not None)
+        return dx, None if mg is not None else dw, None, dout if need[3] else None
+
+
 class SimpleMoE(nn.Module):
     """Dropless top-k MoE FFN with SwiGLU experts in blockwise fp8.
 
@@ -138,6 +204,19 @@ class SimpleMoE(nn.Module):
     scales in the scaled MFMA: the packed-weight GEMMs run
     ``smoe_grouped_gemm_fp8_packed_e8m0`` and the wgrad its E8M0 mode.
 
+    ``recipe="bf16"`` leaves the experts unquantised: rows are permuted as bf16,
+    the products are ``linear_act`` on the bf16 weights (a parameter of another
+    type is converted at each call) and their gradients ``linear_act_bwd``.
+
+    ``shared_intermediate`` adds a dense SwiGLU expert beside the routed ones
+    (``ws1`` [2*Is, H], ``ws2`` [H, Is], bf16 whatever the recipe); its second
+    product adds the routed output in its epilogue.  ``block_norm`` makes the
+    layer a whole pre- and post-normed block: with h = norm(x) * norm_in,
+    forward returns residual_scale * x + block_gate * (norm(layer(h)) *
+    norm_out), each norm an RMS norm over H with ``norm_eps`` and
+    ``norm_in``, ``norm_out``, ``block_gate`` [H] parameters.  Both work under
+    autograd; ``return_intermediates`` is for the routed layer alone.
+
     Under autograd (grad mode on and an input or parameter requiring grad),
     ``forward`` records one graph node whose backward runs the fp8 backward
     (``loss.backward()`` fills w1.grad, w2.grad, w_gate.grad and x.grad).
@@ -154,14 +233,15 @@ class SimpleMoE(nn.Module):
 
     def __init__(self, hidden: int, intermediate: int, num_experts: int, top_k: int,
                  device=None, dtype=torch.bfloat16, router_bias: bool = False,
-                 wgrad_recipe: str = "fp32", recipe: str = "blockwise"):
+                 wgrad_recipe: str = "fp32", recipe: str = "blockwise", shared_intermediate: int = 0,
+                 block_norm: bool = False, residual_scale: float = 1.0, norm_eps: float = 1e-6):
         super().__init__()
         if wgrad_recipe not in ("fp32", "e8m0"):
             raise ValueError("wgrad_recipe is 'fp32' (128x1 scales amax/448) or 'e8m0' "
                              "(power-of-two 128x1 scales applied by the scaled MFMA)")
-        if recipe not in ("blockwise", "e8m0"):
-            raise ValueError("recipe is 'blockwise' (scales amax/448) or 'e8m0' "
-                             "(power-of-two scales for every quantisation)")
+        if recipe not in ("blockwise", "e8m0", "bf16"):
+            raise ValueError("recipe is 'blockwise' (scales amax/448), 'e8m0' "
+                             "(power-of-two scales for every quantisation) or 'bf16' (none)")
         self.wgrad_recipe = wgrad_recipe
         self.recipe = recipe
         self.hidden, self.intermediate = hidden, intermediate
@@ -171,6 +251,14 @@ class SimpleMoE(nn.Module):
         self.w1 = nn.Parameter(torch.empty(num_experts, 2 * intermediate, hidden, **kw))
         self.w2 = nn.Parameter(torch.empty(num_experts, hidden, intermediate, **kw))
         self.register_buffer("router_bias", torch.zeros(num_experts, device=device) if router_bias else None)
+        self.ws1 = self.ws2 = self.norm_in = self.norm_out = self.block_gate = None
+        if shared_intermediate:
+            self.ws1 = nn.Parameter(torch.empty(2 * shared_intermediate, hidden, device=device, dtype=torch.bfloat16))
+            self.ws2 = nn.Parameter(torch.empty(hidden, shared_intermediate, device=device, dtype=torch.bfloat16))
+        self.residual_scale, self.norm_eps = float(residual_scale), float(norm_eps)
+        if block_norm:
+            for name in ("norm_in", "norm_out", "block_gate"):
+                setattr(self, name, nn.Parameter(torch.ones(hidden, **kw)))
         self._fp8 = None
         self._fp8_key = None
         self._gemm = None
@@ -179,7 +267,9 @@ class SimpleMoE(nn.Module):
 
     @torch.no_grad()
     def reset_parameters(self, generator: torch.Generator | None = None, std: float = 0.02):
-        for p in (self.w_gate, self.w1, self.w2):
+        for p in (self.w_gate, self.w1, self.w2, self.ws1, self.ws2):
+            if p is None:
+                continue
             p.copy_(torch.randn(p.shape, generator=generator, dtype=torch.float32,
                                 device=generator.device if generator is not None else p.device).to(p) * std)
 
@@ -267,6 +357,36 @@ class SimpleMoE(nn.Module):
         they are x @ w_gate in fp32.  ``return_intermediates`` returns
         (y, intermediates) for a later ``backward_from`` without recording an
         autograd graph."""
+        if self.ws1 is not None or self.norm_in is not None:
+            if return_intermediates:
+                raise ValueError("return_intermediates is for the routed layer alone: no shared expert, no norms")
+            return self._block_forward(x, logits)
+        return self._routed(x, logits, return_intermediates)
+
+    def _block_forward(self, x, logits):
+        """The routed layer with a shared expert and the block's norms."""
+        x = x.to(torch.bfloat16)
+        norm, scale, eps = self.norm_in is not None, self.residual_scale, self.norm_eps
+        grad = torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, logits, *self.parameters(recurse=False)))
+        h, skip = x, x
+        if norm:
+            x = x.contiguous()
+            h, skip = (_BlockNormIn.apply(x, self.norm_in, eps, scale) if grad
+                       else (block.block_norm_in(x, self.norm_in, eps)[0], x))
+        y = self._routed(h, logits)
+        if self.ws1 is not None:
+            if grad:
+                y = _LinearAct.apply(_LinearAct.apply(h, self.ws1, "swiglu", None), self.ws2, "none", y)
+            else:
+                y = block.linear_act(block.linear_act(h, self.ws1, act="swiglu"), self.ws2, residual=y)
+        if not norm:
+            return y
+        if grad:
+            return _BlockNormOut.apply(y, skip, self.norm_out, self.block_gate, scale, eps)
+        return block.block_norm_out(y, x, self.norm_out, gate=self.block_gate, residual_scale=scale, eps=eps)[0]
+
+    def _routed(self, x, logits=None, return_intermediates: bool = False):
         if return_intermediates:
             with torch.no_grad():
                 if logits is None:
@@ -310,6 +430,8 @@ class SimpleMoE(nn.Module):
             logits = logits.detach().float().contiguous()
         if x.shape[0] == 0:
             return self._empty_forward(x, logits, save)
+        if self.recipe == "bf16":
+            return self._forward_bf16(x, logits, save)
         fp8 = self.fp8_weights()
         w1, w1s, w2, w2s = self._gemm
         K = self.top_k
@@ -384,6 +506,44 @@ class SimpleMoE(nn.Module):
             return out
         return out, dict(x=x, logits=logits, topk_idx=idx, topk_w=w, row_map=row_map, inv_map=inv_map,
                          counts=counts, offsets=off, xq=xq, xs=xs, c1=c1, hq=hq, hs=hs, h=h, y=y, fp8=self._fp8)
+
+    def _bf16_weights(self):
+        return tuple(p.detach().to(torch.bfloat16).contiguous() for p in (self.w1, self.w2))
+
+    def _forward_bf16(self, x, logits, save):
+        """The forward without quantisation (recipe "bf16")."""
+        K = self.top_k
+        if logits is None:
+            logits = ops.gate_logits(x, self.w_gate.detach(), K)
+        w1, w2 = self._bf16_weights()
+        idx, w, row_map, inv_map, counts, off = ops.route_topk_sort(logits, K, self.router_bias)
+        xp = block.permute_tokens_rows(x, inv_map, K)
+        h = block.linear_act(xp, w1, act="swiglu", offsets=off, save_z=save)
+        h, c1 = h if save else (h, None)
+        y = block.linear_act(h, w2, offsets=off)
+        out = block.unpermute_tokens(y, inv_map, K, w)
+        if not save:
+            return out
+        # the weights too: the backward runs on the forward's
+        return out, dict(x=x, logits=logits, topk_idx=idx, topk_w=w, row_map=row_map, inv_map=inv_map, counts=counts,
+                         offsets=off, xp=xp, c1=c1, h=h, y=y, w1=w1, w2=w2)
+
+    def _backward_bf16(self, inter, dout, dw1_into, dw2_into, wgrad_dtype):
+        K, off, inv = self.top_k, inter["offsets"], inter["inv_map"]
+        w1, w2 = inter["w1"], inter["w2"]
+        dw = [into if into is not None else torch.empty(w.shape, dtype=wgrad_dtype, device=w.device)
+              for into, w in ((dw1_into, w1), (dw2_into, w2))]
+        dy, dtw = block.unpermute_tokens_bwd(dout, inv, K, inter["y"], inter["topk_w"])
+        dh, _, _ = block.linear_act_bwd(dy, inter["h"], w2, offsets=off, dw_out=dw[1], accumulate=dw2_into is not None)
+        dxs, _, _ = block.linear_act_bwd(dh, inter["xp"], w1, z=inter["c1"], act="swiglu", offsets=off, dw_out=dw[0],
+                                         accumulate=dw1_into is not None)
+        dx = block.permute_tokens_bwd(dxs, inv, K)
+        dlogits = ops.router_topk_bwd(inter["logits"], inter["topk_idx"], dtw)
+        out = dict(dx=dx, dw1=dw[0], dw2=dw[1], dtopk_w=dtw, dlogits=dlogits, dh=dh, dxs=dxs)
+        if inter.get("logits_from_gate"):
+            out["dx"] = (dx.float() + dlogits @ self.w_gate.detach().t()).to(torch.bfloat16)
+            out["dw_gate"] = inter["x"].float().t() @ dlogits
+        return out
 
     def _layer_flags(self, w1, w2) -> int:
         return ((_C.SMOE_LAYER_W1_PACKED if isinstance(w1, ops.PackedWeight) else 0)
@@ -472,6 +632,8 @@ class SimpleMoE(nn.Module):
             return out
         if (dw1_into is None or dw2_into is None) and wgrad_dtype not in (torch.float32, torch.bfloat16):
             raise TypeError("the weight gradient is fp32 or bf16")
+        if self.recipe == "bf16":
+            return self._backward_bf16(inter, dout.contiguous(), dw1_into, dw2_into, wgrad_dtype)
         w1t, w1ts, w2t, w2ts = self.gemm_weights_t(inter.get("fp8"))
         if not (_weight_is(w1t, w1ts, E, H, 2 * I) and _weight_is(w2t, w2ts, E, I, H)):
             raise ValueError(f"the weights are not those of {E} experts, hidden {H}, intermediate {I}")
