@@ -194,12 +194,12 @@ int linear_rows_blocks(int R, int E);
 bool linear_rows_better(int R, int N, int E, int act);
 int linear_rows(const LinArgs& a, int dtype, hipStream_t s);
 
-// smoe_linear_mm.hip: the tiled kernels, for operands they cover.  what: 0 the
-// product, 1 dx, 2 dW.
-bool linear_mm_ok(const LinArgs& a, int what);
+// The tiled kernels (smoe_linear_mm.h).  what: the product, dx or dW.
+enum { kFwd = 0, kDgrad = 1, kWgrad = 2 };
 // shares that a dense product's sum is cut into, and the bytes of its partial sums
 int linear_mm_splits(int R, int N, int K, int act, int what);
 size_t linear_mm_part_bytes(int R, int N, int K, int act, int what);
-int linear_mm(const LinArgs& a, int what, int dtype, hipStream_t s);
+int linear_mm(LinArgs a, int what, int dtype, hipStream_t s);
+int linear_mm_any(const LinArgs& a, int what, int dtype, hipStream_t s);
 
 }  // namespace smoe

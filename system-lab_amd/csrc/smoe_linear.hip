@@ -15,210 +15,6 @@ namespace smoe {
 
 constexpr int kLinearMaxDim = 1 << 20, kLinearMaxRows = 1 << 29;
 
-// ------------------------------------------------ the product, any sizes ---
-// 64 x 64 tiles, 4 waves of 32 x 32, K in steps of 32 staged through LDS by
-// way of registers.  Rows and columns of any length and alignment.
-enum { kFwd = 0, kDgrad = 1, kWgrad = 2 };
-constexpr int kT = 64, kTK = 32, kPitch = kTK + 8;  // LDS row pitch: 80 bytes
-
-// 8 elements of a row, those past n read as 0 (n may be <= 0).
-template <class T>
-__device__ __forceinline__ v4u_t piece_or_zero(const T* p, int n) {
-  if (n >= 8) return load_piece<T>(p);
-  struct { T v[8]; } b;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) b.v[i] = i < n ? p[i] : T{};
-  return __builtin_bit_cast(v4u_t, b);
-}
-
-// One lane's four neighbouring outputs n .. n + 3 of row m.
-template <class T>
-__device__ __forceinline__ void store4(T* p, int n, const float* f) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < n) p[i] = Elt<T>::from_f32(f[i]);
-}
-template <class T>
-__device__ __forceinline__ float bias_at(const LinArgs& a, size_t i) {
-  return a.bias_f32 ? ((const float*)a.bias)[i] : Elt<T>::to_f32(((const T*)a.bias)[i]);
-}
-
-template <class T, int kAct>
-__device__ __forceinline__ void epilogue4(const LinArgs& a, int e, int m, int n, int cols, float* v, const float* u) {
-  // v: values n .. n+3 of row m (SwiGLU: the gate's, u: the up's), cols: the
-  // output's row length
-  const int left = cols - n;
-  if (left <= 0) return;
-  const size_t nb = (size_t)e * a.N + n;
-  if (a.bias) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) v[i] = v[i] + bias_at<T>(a, nb + i);
-  }
-  float o[4];
-  if constexpr (kAct == SMOE_ACT_SWIGLU) {
-    float w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = u[i];
-      if (a.bias && i < left) w[i] = w[i] + bias_at<T>(a, nb + cols + i);
-      o[i] = act_value<SMOE_ACT_SILU>(v[i]) * w[i];
-    }
-    if (a.z) {
-      store4<T>((T*)a.z + (size_t)m * a.N + n, left, v);
-      store4<T>((T*)a.z + (size_t)m * a.N + cols + n, left, w);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = act_value<kAct>(v[i]);
-    if (a.z) store4<T>((T*)a.z + (size_t)m * a.N + n, left, v);
-  }
-  if (a.residual) {
-    const T* r = (const T*)a.residual + (long long)m * a.ldr + n;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < left) o[i] = o[i] + Elt<T>::to_f32(r[i]);
-  }
-  store4<T>((T*)a.out + (size_t)m * cols + n, left, o);
-}
-
-// kFwd:   D[m][n] = sum_k x[m][k] W[n][k]         rows of the tile's expert
-// kDgrad: D[m][k] = sum_n dz[m][n] W[n][k]        "
-// kWgrad: D[n][k] = sum_r dz[r][n] x[r][k]        over the expert's rows
-// Left and right tiles lie in LDS with the summed index contiguous; operands
-// whose rows run along the other index are turned on the way in.
-template <class T, int kWhat, int kAct>
-__global__ __launch_bounds__(256) void linear_any_kernel(const LinArgs a) {
-  __shared__ __attribute__((aligned(16))) T left[kT * kPitch], right[kT * kPitch];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
-  constexpr bool kPair = kWhat == kFwd && kAct == SMOE_ACT_SWIGLU;
-  const int half = a.N / 2;
-  int e = 0, m0, mrows, n0 = blockIdx.y * kT, ncols, len, k_lo = 0;
-  if constexpr (kWhat == kWgrad) {
-    e = blockIdx.z;
-    m0 = blockIdx.x * kT;
-    mrows = a.N - m0;
-    ncols = a.K;
-    int lo = 0, hi = a.R;
-    if (a.offsets) {
-      lo = clamp_row(a.offsets, e, a.R);
-      hi = clamp_row(a.offsets, e + 1, a.R);
-    }
-    k_lo = lo;
-    len = hi > lo ? hi - lo : 0;
-    if (len == 0 && (a.mode & 1)) return;  // nothing to add
-  } else {
-    RowTile t;
-    if (!find_row_tile<kT>(a.offsets, a.E, a.R, blockIdx.x, &t)) return;
-    e = t.e;
-    m0 = t.row0;
-    mrows = t.rows;
-    ncols = kWhat == kFwd ? (kPair ? half : a.N) : a.K;
-    len = kWhat == kFwd ? a.K : a.N;
-    if (kPair) n0 = blockIdx.y * (kT / 2);
-  }
-  const T* A = (const T*)a.a;
-  const T* B = (const T*)a.b + (kWhat == kWgrad ? 0 : (size_t)e * a.N * a.K);
-  v4f_t acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
-
-  for (int k0 = 0; k0 < len; k0 += kTK) {
-    // 64 rows x 32 k a tile: 256 pieces of 8, one a thread
-    const int r = tid >> 2, c = (tid & 3) * 8;       // row-wise: row r, k = c ..
-    const int kr = tid >> 3, cr = (tid & 7) * 8;     // turned: k = kr, rows cr ..
-    v4u_t pa, pb;
-    if constexpr (kWhat != kWgrad) {
-      const int row = r < mrows ? m0 + r : m0;
-      pa = piece_or_zero<T>(A + (long long)row * a.lda + k0 + c, r < mrows ? len - k0 - c : 0);
-    } else {
-      const int row = k_lo + (k0 + kr < len ? k0 + kr : 0);
-      pa = piece_or_zero<T>(A + (long long)row * a.lda + m0 + cr, k0 + kr < len ? mrows - cr : 0);
-    }
-    if constexpr (kWhat == kFwd) {
-      int n = n0 + r, ok = n < ncols;
-      if constexpr (kPair) {  // 16 gate rows, 16 up rows, alternately
-        n = n0 + (r >> 5) * 16 + (r & 15);
-        ok = n < half;
-        n += (r & 16) ? half : 0;
-      }
-      pb = piece_or_zero<T>(B + (size_t)(ok ? n : 0) * a.K + k0 + c, ok ? len - k0 - c : 0);
-    } else if constexpr (kWhat == kDgrad) {
-      const int n = k0 + kr;
-      pb = piece_or_zero<T>(B + (size_t)(n < len ? n : 0) * a.K + n0 + cr, n < len ? ncols - n0 - cr : 0);
-    } else {
-      const int row = k_lo + (k0 + kr < len ? k0 + kr : 0);
-      pb = piece_or_zero<T>(B + (long long)row * a.ldb + n0 + cr, k0 + kr < len ? ncols - n0 - cr : 0);
-    }
-    __syncthreads();
-    auto turn = [&](T* t, const v4u_t& p) {
-      struct B { T v[8]; };
-      const B b = __builtin_bit_cast(B, p);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[(cr + i) * kPitch + kr] = b.v[i];
-    };
-    if constexpr (kWhat != kWgrad) *(v4u_t*)(left + r * kPitch + c) = pa;
-    else turn(left, pa);
-    if constexpr (kWhat == kFwd) *(v4u_t*)(right + r * kPitch + c) = pb;
-    else turn(right, pb);
-    __syncthreads();
-    v4u_t fa[2], fb[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      fa[i] = *(const v4u_t*)(left + (wm + i * 16 + (lane & 15)) * kPitch + (lane >> 4) * 8);
-      fb[i] = *(const v4u_t*)(right + (wn + i * 16 + (lane & 15)) * kPitch + (lane >> 4) * 8);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma32<T>(fb[j], fa[i], acc[i][j]);
-  }
-
-  // the right operand went in first: a lane holds four neighbouring columns
-  const int mi = lane & 15, nq = (lane >> 4) * 4;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int m = wm + i * 16 + mi;
-    if (m >= mrows) continue;
-    if constexpr (kWhat == kFwd) {
-      if constexpr (kPair) {
-        epilogue4<T, kAct>(a, e, m0 + m, n0 + wn / 2 + nq, half, (float*)&acc[i][0], (const float*)&acc[i][1]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          epilogue4<T, kAct>(a, e, m0 + m, n0 + wn + j * 16 + nq, a.N, (float*)&acc[i][j], nullptr);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int n = n0 + wn + j * 16 + nq;
-        const int n_left = ncols - n;
-        if (n_left <= 0) continue;
-        float* v = (float*)&acc[i][j];
-        if constexpr (kWhat == kDgrad) {
-          store4<T>((T*)a.out + (size_t)(m0 + m) * a.K + n, n_left, v);
-        } else {
-          const size_t at = ((size_t)e * a.N + m0 + m) * a.K + n;
-          if (a.mode < 2) {
-            float* d = (float*)a.out + at;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (q < n_left) d[q] = (a.mode & 1) ? d[q] + v[q] : v[q];
-          } else {
-            T* d = (T*)a.out + at;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (q < n_left) d[q] = Elt<T>::from_f32((a.mode & 1) ? Elt<T>::to_f32(d[q]) + v[q] : v[q]);
-          }
-        }
-      }
-    }
-  }
-}
-
 // ------------------------------------------- dz and the biases' gradient ---
 // Rows in blocks of 64 of one expert; a thread owns 8 columns (SwiGLU: 8 gate
 // columns and their 8 up columns), 32 threads side by side and 8 rows at a
@@ -338,19 +134,8 @@ static int row_tiles(int R, int E, int bm) { return (R + bm - 1) / bm + E - 1; }
     }                                                                  \
   } while (0)
 
-template <class T>
-static int linear_fwd(const LinArgs& a, hipStream_t s) {
-  const bool tiled = linear_mm_ok(a, kFwd);
-  if (tiled ? linear_rows_better(a.R, a.N, a.E, a.act) : linear_rows_blocks(a.R, a.E) != 0)
-    return linear_rows(a, Elt<T>::kDtype, s);
-  if (tiled) return linear_mm(a, kFwd, Elt<T>::kDtype, s);
-  const int act = a.act;
-  const int cols = act == SMOE_ACT_SWIGLU ? a.N / 2 : a.N, bn = act == SMOE_ACT_SWIGLU ? kT / 2 : kT;
-  const dim3 grid(row_tiles(a.R, a.E, kT), (cols + bn - 1) / bn);
-#define SMOE_LF(A) linear_any_kernel<T, kFwd, A><<<grid, dim3(256), 0, s>>>(a)
-  SMOE_LIN_ACTS(SMOE_LF);
-#undef SMOE_LF
-  SMOE_RETURN_LAUNCH();
+static int linear_fwd(const LinArgs& a, int dtype, hipStream_t s) {
+  return linear_rows_better(a.R, a.N, a.E, a.act) ? linear_rows(a, dtype, s) : linear_mm(a, kFwd, dtype, s);
 }
 
 // Parts of the gradients' workspace, each a multiple of 256 bytes.
@@ -389,20 +174,13 @@ static int linear_bwd(const smoe_linear_bwd& q, hipStream_t s) {
   const long long lddz = has_act ? q.N : q.lddout;
   if (q.dx) {
     const LinArgs a{dz, q.w, lddz, q.K, nullptr, nullptr, 0, q.offsets, q.dx, nullptr, q.E, q.R, q.N, q.K, 0, 0, 0, cut, 1};
-    if (linear_mm_ok(a, kDgrad)) {
-      const int st = linear_mm(a, kDgrad, q.dtype, s);
-      if (st) return st;
-    } else {
-      linear_any_kernel<T, kDgrad, SMOE_ACT_NONE>
-          <<<dim3(row_tiles(q.R, q.E, kT), (q.K + kT - 1) / kT), dim3(256), 0, s>>>(a);
-    }
+    const int st = linear_mm(a, kDgrad, q.dtype, s);
+    if (st) return st;
   }
   if (q.dw) {
     const LinArgs a{dz, q.x, lddz, q.ldx, nullptr, nullptr, 0, q.offsets, q.dw, nullptr, q.E, q.R, q.N, q.K, 0, 0,
                     q.dw_mode, cut, 1};
-    if (linear_mm_ok(a, kWgrad)) return linear_mm(a, kWgrad, q.dtype, s);
-    linear_any_kernel<T, kWgrad, SMOE_ACT_NONE>
-        <<<dim3((q.N + kT - 1) / kT, (q.K + kT - 1) / kT, q.E), dim3(256), 0, s>>>(a);
+    return linear_mm(a, kWgrad, q.dtype, s);
   }
   SMOE_RETURN_LAUNCH();
 }
@@ -446,7 +224,7 @@ extern "C" int smoe_linear_act(const smoe_linear_fwd* q, void* stream) {
   const LinArgs a{q->x, q->w, q->ldx, q->K, q->bias, q->residual, q->ldr, q->offsets, q->out, q->z,
                   q->E, q->R, q->N, q->K, q->bias_f32, q->act, 0, need ? (float*)q->ws : nullptr, 1};
   hipStream_t s = (hipStream_t)stream;
-  return q->dtype == SMOE_BF16 ? linear_fwd<bf16_t>(a, s) : linear_fwd<f16_t>(a, s);
+  return linear_fwd(a, q->dtype, s);
 }
 
 extern "C" size_t smoe_linear_act_bwd_workspace_size(int R, int N, int K, int E, int act, int with_bias) {
