@@ -490,116 +490,137 @@ __global__ __launch_bounds__(C::kThreads, 2) void linear_mm_kernel(const LinArgs
 
   // ---- epilogue -------------------------------------------------------------
   // A lane holds rows 16 i + lane % 16 of its wave's and kRuns runs of 8
-  // columns, 32 columns apart.
+  // columns, 32 columns apart: both runs of a row are stored one after the
+  // other, a whole 128-byte line (runs in the outer loop, half lines a pass,
+  // took 9 us longer a round of dW tiles' 128 KiB).
   constexpr int kRuns = kPair ? 1 : 2;
-  auto store = [&](const MmTile& t) {
-    if (kWhat == kWgrad && t.len == 0 && (a.mode & 1)) return;  // nothing to add
+  // a cut sum's share as it is; mm_join_kernel does the rest
+  auto store_share = [&](const MmTile& t) {
+    const size_t width = kPair ? a.N : cols;
+    float* part = a.part + (size_t)blockIdx.y * (kWhat == kWgrad ? a.N : a.R) * width;
+#pragma unroll
+    for (int i = 0; i < kRB; ++i) {
+      const int m = wr * kRB * 16 + i * 16 + (lane & 15);
+      if (m >= t.mrows) continue;
+#pragma unroll
+      for (int p = 0; p < kRuns; ++p) {
+        const int n = t.n0 + wn * (kPair ? 32 : 64) + g * 8 + p * 32, np = t.n0 + t.ncols - n;
+        float* d = part + (size_t)(t.m0 + m) * width + n;
+#pragma unroll
+        for (int j = 0; j < kCB / kRuns; ++j) {
+          const int c = (kPair ? j >> 1 : j) * 4;
+          if (c < np)
+            store_f32<float>(d + c + (kPair && (j & 1) ? cols : 0), np - c, (const float*)&acc[i][p * 2 + j]);
+        }
+      }
+    }
+  };
+  auto store_fwd = [&](const MmTile& t) {
     const int n0 = t.n0 + wn * (kPair ? 32 : 64) + g * 8;
+    float b0[kRuns][8], b1[8];
 #pragma unroll
     for (int p = 0; p < kRuns; ++p) {
-      const int n = n0 + p * 32, np = t.n0 + t.ncols - n;  // columns of the run that exist
-      if (np <= 0) break;
-      if (a.splits > 1) {  // the share's sums as they are; mm_join_kernel does the rest
-        const size_t width = kPair ? a.N : cols;
-        float* part = a.part + (size_t)blockIdx.y * (kWhat == kWgrad ? a.N : a.R) * width + n;
+      const int n = n0 + p * 32, np = t.n0 + t.ncols - n;
 #pragma unroll
-        for (int i = 0; i < kRB; ++i) {
-          const int m = wr * kRB * 16 + i * 16 + (lane & 15);
-          if (m >= t.mrows) continue;
-          float* d = part + (size_t)(t.m0 + m) * width;
-#pragma unroll
-          for (int j = 0; j < kCB / kRuns; ++j) {
-            const int c = (kPair ? j >> 1 : j) * 4;
-            if (c < np)
-              store_f32<float>(d + c + (kPair && (j & 1) ? cols : 0), np - c, (const float*)&acc[i][p * 2 + j]);
-          }
-        }
-        continue;
+      for (int x = 0; x < 8; ++x) b0[p][x] = b1[x] = 0.0f;
+      if (a.bias && np > 0) {
+        load_param<T>(a.bias, a.bias_f32, (size_t)t.e * a.N + n, np, b0[p]);
+        if constexpr (kPair) load_param<T>(a.bias, a.bias_f32, (size_t)t.e * a.N + cols + n, np, b1);
       }
-      float b0[8], b1[8];
-      v4u_t res[kRB];
-      const bool whole = kWhat == kFwd && a.residual && np >= 8;
-      if constexpr (kWhat == kFwd) {
+    }
+    constexpr int kAhead = 4;  // rows whose residuals are in flight together
+    v4u_t res[kAhead][kRuns];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) b0[i] = b1[i] = 0.0f;
-        if (a.bias) {
-          load_param<T>(a.bias, a.bias_f32, (size_t)t.e * a.N + n, np, b0);
-          if constexpr (kPair) load_param<T>(a.bias, a.bias_f32, (size_t)t.e * a.N + cols + n, np, b1);
-        }
-        if (whole) {  // all rows' residuals in flight together
+    for (int i = 0; i < kRB; ++i) {
+      if (a.residual && i % kAhead == 0) {
 #pragma unroll
-          for (int i = 0; i < kRB; ++i) {
-            const int m = wr * kRB * 16 + i * 16 + (lane & 15);
-            res[i] = load_piece<T>((const T*)a.residual +
-                                   (long long)(t.m0 + (m < t.mrows ? m : t.mrows - 1)) * a.ldr + n);
-          }
+        for (int q = 0; q < kAhead; ++q) {
+          const int m = wr * kRB * 16 + (i + q) * 16 + (lane & 15);
+          const T* r = (const T*)a.residual + (long long)(t.m0 + (m < t.mrows ? m : t.mrows - 1)) * a.ldr + n0;
+#pragma unroll
+          for (int p = 0; p < kRuns; ++p)
+            if (n0 + p * 32 + 8 <= t.n0 + t.ncols) res[q][p] = load_piece<T>(r + p * 32);
         }
       }
+      const int m = wr * kRB * 16 + i * 16 + (lane & 15);
+      if (m >= t.mrows) continue;
+      const size_t row = (size_t)t.m0 + m;
 #pragma unroll
-      for (int i = 0; i < kRB; ++i) {
-        const int m = wr * kRB * 16 + i * 16 + (lane & 15);
-        if (m >= t.mrows) continue;
-        const size_t row = (size_t)t.m0 + m;
+      for (int p = 0; p < kRuns; ++p) {
+        const int n = n0 + p * 32, np = t.n0 + t.ncols - n;  // columns of the run that exist
+        if (np <= 0) break;
         float v[8];
-        if constexpr (kWhat == kFwd) {
-          if constexpr (kPair) {
-            float u[8];
+        if constexpr (kPair) {
+          float u[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              v[x] = acc[i][x / 4 * 2][x & 3] + b0[x];
-              u[x] = acc[i][x / 4 * 2 + 1][x & 3] + b1[x];
-            }
-            if (a.z) {
-              store_f32<T>((T*)a.z + row * a.N + n, np, v);
-              store_f32<T>((T*)a.z + row * a.N + cols + n, np, u);
-            }
-#pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] = act_value<SMOE_ACT_SILU>(v[x]) * u[x];
-          } else {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] = acc[i][p * 2 + x / 4][x & 3] + b0[x];
-            if (a.z) store_f32<T>((T*)a.z + row * a.N + n, np, v);
-#pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] = act_value<kAct>(v[x]);
+          for (int x = 0; x < 8; ++x) {
+            v[x] = acc[i][x / 4 * 2][x & 3] + b0[p][x];
+            u[x] = acc[i][x / 4 * 2 + 1][x & 3] + b1[x];
           }
-          if (a.residual) {
-            float r[8];
-            if (whole) Elt<T>::unpack(res[i], r);
-            else load_f32<T>((const T*)a.residual + (long long)row * a.ldr + n, np, r);
-#pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] = v[x] + r[x];
+          if (a.z) {
+            store_f32<T>((T*)a.z + row * a.N + n, np, v);
+            store_f32<T>((T*)a.z + row * a.N + cols + n, np, u);
           }
-          store_f32<T>((T*)a.out + row * cols + n, np, v);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[x] = act_value<SMOE_ACT_SILU>(v[x]) * u[x];
         } else {
 #pragma unroll
-          for (int x = 0; x < 8; ++x) v[x] = acc[i][p * 2 + x / 4][x & 3];
-          if constexpr (kWhat == kDgrad) {
-            store_f32<T>((T*)a.out + row * cols + n, np, v);
-          } else {
-            const size_t at = ((size_t)t.e * a.N + row) * cols + n;
-            if (a.mode < 2) {
-              float* d = (float*)a.out + at;
+          for (int x = 0; x < 8; ++x) v[x] = acc[i][p * 2 + x / 4][x & 3] + b0[p][x];
+          if (a.z) store_f32<T>((T*)a.z + row * a.N + n, np, v);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                if (np <= 4 * h) break;
-                float w[4];
-                if (a.mode & 1) {
-                  load_f32<float>(d + 4 * h, np - 4 * h, w);
+          for (int x = 0; x < 8; ++x) v[x] = act_value<kAct>(v[x]);
+        }
+        if (a.residual) {
+          float r[8];
+          if (np >= 8) Elt<T>::unpack(res[i % kAhead][p], r);
+          else load_f32<T>((const T*)a.residual + (long long)row * a.ldr + n, np, r);
 #pragma unroll
-                  for (int x = 0; x < 4; ++x) v[4 * h + x] = w[x] + v[4 * h + x];
-                }
-                store_f32<float>(d + 4 * h, np - 4 * h, v + 4 * h);
-              }
-            } else {
-              T* d = (T*)a.out + at;
+          for (int x = 0; x < 8; ++x) v[x] = v[x] + r[x];
+        }
+        store_f32<T>((T*)a.out + row * cols + n, np, v);
+      }
+    }
+  };
+  auto store_grad = [&](const MmTile& t) {
+    if (kWhat == kWgrad && t.len == 0 && (a.mode & 1)) return;  // nothing to add
+#pragma unroll
+    for (int i = 0; i < kRB; ++i) {
+      const int m = wr * kRB * 16 + i * 16 + (lane & 15);
+      if (m >= t.mrows) continue;
+      const size_t row = (size_t)t.m0 + m;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int n = t.n0 + wn * 64 + g * 8 + p * 32, np = t.n0 + t.ncols - n;
+        if (np <= 0) break;
+        float v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = acc[i][p * 2 + x / 4][x & 3];
+        if constexpr (kWhat == kDgrad) {
+          store_f32<T>((T*)a.out + row * cols + n, np, v);
+        } else {
+          const size_t at = ((size_t)t.e * a.N + row) * cols + n;
+          if (a.mode < 2) {
+            float* d = (float*)a.out + at;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (np <= 4 * h) break;
+              float w[4];
               if (a.mode & 1) {
-                float w[8];
-                load_f32<T>(d, np, w);
+                load_f32<float>(d + 4 * h, np - 4 * h, w);
 #pragma unroll
-                for (int x = 0; x < 8; ++x) v[x] = w[x] + v[x];
+                for (int x = 0; x < 4; ++x) v[4 * h + x] = w[x] + v[4 * h + x];
               }
-              store_f32<T>(d, np, v);
+              store_f32<float>(d + 4 * h, np - 4 * h, v + 4 * h);
             }
+          } else {
+            T* d = (T*)a.out + at;
+            if (a.mode & 1) {
+              float w[8];
+              load_f32<T>(d, np, w);
+#pragma unroll
+              for (int x = 0; x < 8; ++x) v[x] = w[x] + v[x];
+            }
+            store_f32<T>(d, np, v);
           }
         }
       }
@@ -624,7 +645,9 @@ __global__ __launch_bounds__(C::kThreads, 2) void linear_mm_kernel(const LinArgs
       setup(cur);
       start();
     }
-    store(done);
+    if (a.splits > 1) store_share(done);
+    else if constexpr (kWhat == kFwd) store_fwd(done);
+    else store_grad(done);
   }
 }
 
