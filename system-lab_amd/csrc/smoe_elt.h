@@ -113,6 +113,17 @@ __device__ __forceinline__ void store_f32(T* p, int n, const float* f) {
   }
 }
 
+// The same as a raw piece.
+template <class T>
+__device__ __forceinline__ v4u_t load_some(const T* p, int n) {
+  constexpr int V = Elt<T>::kVec;
+  if (n >= V) return load_piece<T>(p);
+  struct { T v[V]; } b;
+#pragma unroll
+  for (int i = 0; i < V; ++i) b.v[i] = i < n ? p[i] : T{};
+  return __builtin_bit_cast(v4u_t, b);
+}
+
 // A parameter vector in the operands' type T or in fp32.
 template <class T>
 __device__ __forceinline__ void load_param(const void* p, bool f32, size_t i, int n, float* f) {

@@ -114,7 +114,16 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* part, const
   }
   if (c >= N) return;
   float s = 0.0f;
-  for (int b = 0; b < count; ++b) s = s + part[(size_t)(first + b) * N + c];
+  int b = 0;
+  const float* p = part + (size_t)first * N + c;
+  for (; b + 8 <= count; b += 8) {  // eight rows in flight, added in order
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p[(size_t)(b + i) * N];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = s + v[i];
+  }
+  for (; b < count; ++b) s = s + p[(size_t)b * N];
   if (f32) ((float*)db)[(size_t)e * N + c] = s;
   else ((T*)db)[(size_t)e * N + c] = Elt<T>::from_f32(s);
 }

@@ -79,16 +79,6 @@ __device__ __forceinline__ int swz_right(int k) { return (k & 3) << 2; }
 // writes 64 contiguous bytes of 16 rows.
 __device__ __forceinline__ int col_of(int j, int r) { return (j >> 1) * 32 + (r >> 2) * 8 + (j & 1) * 4 + (r & 3); }
 
-// The first n (0 at least) of 8 elements, the others 0.
-template <class T>
-__device__ __forceinline__ v4u_t some_piece(const T* p, int n) {
-  if (n >= 8) return load_piece<T>(p);
-  struct { T v[8]; } b;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) b.v[i] = i < n ? p[i] : T{};
-  return __builtin_bit_cast(v4u_t, b);
-}
-
 // One output tile: rows m0 .. + mrows, columns n0 .. + ncols of expert e, the
 // sum over len terms from `lo` (kWgrad: the expert's first row; cut sums: the
 // share's first step).
@@ -312,10 +302,10 @@ __global__ __launch_bounds__(C::kThreads, 2) void linear_mm_kernel(const LinArgs
       const uint8_t* base = a_base + s * sa;
       if constexpr (kTurnA) {
         turn_seg(wid * kASegs + j, kBM, &term, &x);
-        ra_[j] = some_piece<T>((const T*)(base + (size_t)term * pa) + oa[j], term < left ? la[j] : 0);
+        ra_[j] = load_some<T>((const T*)(base + (size_t)term * pa) + oa[j], term < left ? la[j] : 0);
       } else {
         row_seg(wid * kASegs + j, &x, &term);
-        ra_[j] = some_piece<T>((const T*)(base + (size_t)oa[j] * pa) + term * 8, left - term * 8);
+        ra_[j] = load_some<T>((const T*)(base + (size_t)oa[j] * pa) + term * 8, left - term * 8);
       }
     }
 #pragma unroll
@@ -323,10 +313,10 @@ __global__ __launch_bounds__(C::kThreads, 2) void linear_mm_kernel(const LinArgs
       const uint8_t* base = b_base + s * sb;
       if constexpr (kTurnB) {
         turn_seg(wid * kBSegs + j, kBN, &term, &x);
-        rb_[j] = some_piece<T>((const T*)(base + (size_t)term * pb) + ob[j], term < left ? lb[j] : 0);
+        rb_[j] = load_some<T>((const T*)(base + (size_t)term * pb) + ob[j], term < left ? lb[j] : 0);
       } else {
         row_seg(wid * kBSegs + j, &x, &term);
-        rb_[j] = some_piece<T>((const T*)(base + (size_t)ob[j] * pb) + term * 8, left - term * 8);
+        rb_[j] = load_some<T>((const T*)(base + (size_t)ob[j] * pb) + term * 8, left - term * 8);
       }
     }
   };

@@ -19,16 +19,6 @@ namespace smoe {
 
 constexpr int kRowsWaves = 8;
 
-// 8 elements of a row, those past n read as 0.
-template <class T>
-__device__ __forceinline__ v4u_t tail_piece(const T* p, int n) {
-  if (n >= 8) return load_piece<T>(p);
-  struct { T v[8]; } b;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) b.v[i] = i < n ? p[i] : T{};
-  return __builtin_bit_cast(v4u_t, b);
-}
-
 template <class T, int kMB, int kNB, int kU, int kAct>
 __global__ __launch_bounds__(512, 2) void linear_rows_kernel(const LinArgs a) {
   constexpr bool kPair = kAct == SMOE_ACT_SWIGLU;
@@ -91,9 +81,9 @@ __global__ __launch_bounds__(512, 2) void linear_rows_kernel(const LinArgs a) {
       const int k = u * 64 + h * 32, n = K - k - c;  // terms from this lane's first
       v4u_t fw[kNB], fx[kMB];
 #pragma unroll
-      for (int j = 0; j < kNB; ++j) fw[j] = tail_piece<T>(wr[j] + k, n);
+      for (int j = 0; j < kNB; ++j) fw[j] = load_some<T>(wr[j] + k, n);
 #pragma unroll
-      for (int i = 0; i < kMB; ++i) fx[i] = tail_piece<T>(xr[i] + k, n);
+      for (int i = 0; i < kMB; ++i) fx[i] = load_some<T>(xr[i] + k, n);
 #pragma unroll
       for (int i = 0; i < kMB; ++i)
 #pragma unroll

@@ -371,14 +371,15 @@ static int check_norm(int T, int H, int dtype, int gate_mode, int param_f32) {
   return SMOE_OK;
 }
 
-// kNV for a row of H at `waves` waves: the next of 1, 2, 4, 8, 16.
-#define SMOE_NORM_NV(need, CALL) \
-  do {                           \
-    if ((need) <= 1) CALL(1);    \
-    else if ((need) <= 2) CALL(2); \
-    else if ((need) <= 4) CALL(4); \
-    else if ((need) <= 8) CALL(8); \
-    else CALL(16);               \
+// kNV for a row of H at `waves` waves: the next of 1, 2, 4, 8, and for fp32,
+// whose pieces hold half as many values, 16.
+#define SMOE_NORM_NV(need, CALL)                           \
+  do {                                                     \
+    if ((need) <= 1) CALL(1);                              \
+    else if ((need) <= 2) CALL(2);                         \
+    else if ((need) <= 4) CALL(4);                         \
+    else if (V == 8 || (need) <= 8) CALL(8);               \
+    else CALL((V == 4 ? 16 : 8));                          \
   } while (0)
 
 template <class T, bool kOut>
@@ -431,8 +432,8 @@ static int norm_bwd_launch(NormBwd a, void* dweight, void* dgate_ch, hipStream_t
     else norm_bwd_kernel<T, 6, 512, -1><<<grid, block, lds, s>>>(a);
   } else {
     if (need <= 4) norm_bwd_kernel<T, 4, 1024, -1><<<grid, block, lds, s>>>(a);
-    else if (need <= 8) norm_bwd_kernel<T, 8, 1024, -1><<<grid, block, lds, s>>>(a);
-    else norm_bwd_kernel<T, 16, 1024, -1><<<grid, block, lds, s>>>(a);
+    else if (V == 8 || need <= 8) norm_bwd_kernel<T, 8, 1024, -1><<<grid, block, lds, s>>>(a);
+    else norm_bwd_kernel<T, V == 4 ? 16 : 8, 1024, -1><<<grid, block, lds, s>>>(a);
   }
 #undef SMOE_NBG
 #undef SMOE_NB

@@ -62,40 +62,52 @@ __global__ __launch_bounds__(1024) void tokens_kernel(const TokArgs a) {
       const int n = H - c;
       float x[V];
       if constexpr (kScatter || kDot) load_f32<T>(tok + c, n, x);
+      // the expert rows eight at a time: eight loads in flight
+      constexpr int kG = kMaxK < 8 ? kMaxK : 8;
       if constexpr (kScatter) {
         T* dst = (T*)a.out;
-        float y[kDot ? kMaxK : 1][V];
-        if constexpr (kDot) {
 #pragma unroll
-          for (int k = 0; k < kMaxK; ++k)
-            if (r[k] >= 0) load_f32<T>(rows + (long long)r[k] * a.ld_rows + c, n, y[k]);
-        }
+        for (int k0 = 0; k0 < kMaxK; k0 += kG) {
+          v4u_t p[kDot ? kG : 1];
+          if constexpr (kDot) {
 #pragma unroll
-        for (int k = 0; k < kMaxK; ++k) {
-          if (r[k] >= 0) {
-            float o[V];
+            for (int k = 0; k < kG; ++k)
+              if (r[k0 + k] >= 0) p[k] = load_some<T>(rows + (long long)r[k0 + k] * a.ld_rows + c, n);
+          }
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              o[i] = wk[k] * x[i];
-              if constexpr (kDot) dot[k] = __builtin_fmaf(x[i], y[k][i], dot[k]);
+          for (int k = 0; k < kG; ++k) {
+            if (r[k0 + k] >= 0) {
+              float o[V], y[V];
+              if constexpr (kDot) Elt<T>::unpack(p[k], y);
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                o[i] = wk[k0 + k] * x[i];
+                if constexpr (kDot) dot[k0 + k] = __builtin_fmaf(x[i], y[i], dot[k0 + k]);
+              }
+              store_f32<T>(dst + (size_t)r[k0 + k] * H + c, n, o);
             }
-            store_f32<T>(dst + (size_t)r[k] * H + c, n, o);
           }
         }
       } else {
-        float y[kMaxK][V], acc[V];
-#pragma unroll
-        for (int k = 0; k < kMaxK; ++k)
-          if (r[k] >= 0) load_f32<T>(rows + (long long)r[k] * a.ld_rows + c, n, y[k]);
+        float acc[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kMaxK; ++k) {
-          if (r[k] >= 0) {
+        for (int k0 = 0; k0 < kMaxK; k0 += kG) {
+          v4u_t p[kG];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              acc[i] = __builtin_fmaf(wk[k], y[k][i], acc[i]);
-              if constexpr (kDot) dot[k] = __builtin_fmaf(x[i], y[k][i], dot[k]);
+          for (int k = 0; k < kG; ++k)
+            if (r[k0 + k] >= 0) p[k] = load_some<T>(rows + (long long)r[k0 + k] * a.ld_rows + c, n);
+#pragma unroll
+          for (int k = 0; k < kG; ++k) {
+            if (r[k0 + k] >= 0) {
+              float y[V];
+              Elt<T>::unpack(p[k], y);
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                acc[i] = __builtin_fmaf(wk[k0 + k], y[i], acc[i]);
+                if constexpr (kDot) dot[k0 + k] = __builtin_fmaf(x[i], y[i], dot[k0 + k]);
+              }
             }
           }
         }
