@@ -714,7 +714,8 @@ int smoe_layer_backward(const smoe_layer_bwd* args, void* stream, void* side_str
  * size, and "ld" arguments are the elements between an input's rows (outputs
  * and weights are dense).  Row lengths need not be multiples of anything.
  * No counterpart in the reference beyond the dataflow each one serves:
- * dispatch and combine (moe/MoE_detailed_computation_dataflow.md:94-116,195),
+ * dispatch and combine (moe/MegatronCore_MoE_reading_notes.md:94-99,
+ * moe/MoE_detailed_computation_dataflow.md:195),
  * expert products (moe/MegatronCore_MoE_reading_notes.md:84-116).
  */
 #define SMOE_BF16 0
@@ -794,7 +795,8 @@ int smoe_block_norm_out_bwd(const void* dout, long long lddout, const void* y, l
  * [0, R); rows in no expert's range are not written.  act SMOE_ACT_SWIGLU
  * takes W's rows as gate | up halves: out = silu(gate) up, N/2 columns.
  * z [R,N] (may be NULL) receives x W^T + bias for the backward pass.
- * R <= 2^29, N and K <= 2^20.
+ * R <= 2^29, N and K <= 2^20.  ws must hold smoe_linear_act_workspace_size()
+ * bytes (0 where the product needs none).
  *
  * The gradients, dz = dout act'(z) (z may be NULL for SMOE_ACT_NONE):
  * dx = dz W, dw = dz^T x per expert, dbias = sum of dz; each output may be
