@@ -18,11 +18,11 @@ static bool mm_aligned(const LinArgs& a, int what) {
 }
 
 // Big tiles need rows to fill them and as many tiles as compute units; small
-// ones run two workgroups a unit.  us big / small, K 4096, N 4096, no
-// experts: R 4096 106 / 134, R 2048 93 / 79, R 512 79 / 51; K 2048, N 1536, 128
-// experts: R 65536 528 / 615, R 16384 246 / 230, R 8192 223 / 188; dx of the
-// same: 485 / 623, 237 / 239, 218 / 193.  dW, whose tiles do not depend on the
-// rows: K = N = 4096 242 / 303 at R 8192, 31 / 30 at 512, 20 / 16 at 128.
+// ones run two workgroups a unit.  us big / small, K 4096, N 4096, no experts:
+// R 4096 121 / 154, R 3000 95 / 108, R 2048 83 / 64; K 2048, N 1536, 128 experts:
+// R 65536 528 / 613, R 32768 310 / 338, R 16384 249 / 224; dx of the same 483 /
+// 655, 296 / 363, 239 / 237.  dW's tiles do not depend on the rows: of 4096 x 4096
+// 121 / 146 at R 4096, 59 / 78 at R 2048, of 2048 x 2048 (64 tiles) 175 / 99.
 static bool mm_big(const LinArgs& a, int what) {
   const int cols = what == kFwd && a.act == SMOE_ACT_SWIGLU ? a.N / 2 : what == kFwd ? a.N : a.K;
   const int bn = what == kFwd && a.act == SMOE_ACT_SWIGLU ? 128 : 256;
@@ -34,8 +34,8 @@ static bool mm_big(const LinArgs& a, int what) {
 
 // A dense product of few tiles cuts its sum into shares that fill the chip
 // (with experts there are tiles enough, or too few rows to matter).  The model:
-// a round of small tiles takes about 0.8 us a step with one workgroup a unit and
-// 1.25 with two; the shares' fp32 sums are written and read at 4 TB/s and
+// a round of small tiles takes about 0.75 us a step with one workgroup a unit and
+// 1.0 with two; the shares' fp32 sums are written and read at 4 TB/s and
 // joined in a launch of their own (4 us).
 int linear_mm_splits(int R, int N, int K, int act, int what) {
   const bool pair = what == kFwd && act == SMOE_ACT_SWIGLU;
@@ -45,10 +45,10 @@ int linear_mm_splits(int R, int N, int K, int act, int what) {
   const double steps = (double)((len + kStep - 1) / kStep);
   if (tiles >= 256 || rows > 65535) return 1;
   int best = 1;
-  double least = steps * 0.8;
+  double least = steps * 0.75;
   for (int s = 2; s <= 16 && s * 4 <= steps; s *= 2) {
     const long long wgs = tiles * s;
-    const double round = wgs <= 256 ? 0.8 : 1.25 * (double)((wgs + 511) / 512);
+    const double round = wgs <= 256 ? 0.75 : 1.0 * (double)((wgs + 511) / 512);
     const double t = round * steps / s + 4.0 + (double)s * rows * width * 8.0 / 4e6;
     if (t < least) {
       least = t;

@@ -102,6 +102,12 @@ class _GateLinear(torch.autograd.Function):
         return dx, dw, None
 
 
+def _operand(p: torch.Tensor, *dtypes) -> torch.Tensor:
+    """A parameter in a type the operators take (a module converted to another
+    type is converted at each call, as the experts' weights are)."""
+    return p if p.dtype in dtypes else p.to(dtypes[0])
+
+
 def _rows_grad(g: torch.Tensor) -> torch.Tensor:
     """A gradient as the operators take it: autograd may hand over an expanded
     one, or one of other strides."""
@@ -258,7 +264,8 @@ class SimpleMoE(nn.Module):
         self.residual_scale, self.norm_eps = float(residual_scale), float(norm_eps)
         if block_norm:
             for name in ("norm_in", "norm_out", "block_gate"):
-                setattr(self, name, nn.Parameter(torch.ones(hidden, **kw)))
+                setattr(self, name, nn.Parameter(torch.ones(
+                    hidden, device=device, dtype=dtype if dtype == torch.bfloat16 else torch.float32)))
         self._fp8 = None
         self._fp8_key = None
         self._gemm = None
@@ -372,19 +379,22 @@ class SimpleMoE(nn.Module):
         h, skip = x, x
         if norm:
             x = x.contiguous()
-            h, skip = (_BlockNormIn.apply(x, self.norm_in, eps, scale) if grad
-                       else (block.block_norm_in(x, self.norm_in, eps)[0], x))
+            n1, n2, gate = (_operand(p, torch.float32, torch.bfloat16)
+                            for p in (self.norm_in, self.norm_out, self.block_gate))
+            h, skip = (_BlockNormIn.apply(x, n1, eps, scale) if grad
+                       else (block.block_norm_in(x, n1, eps)[0], x))
         y = self._routed(h, logits)
         if self.ws1 is not None:
+            ws1, ws2 = (_operand(p, torch.bfloat16) for p in (self.ws1, self.ws2))
             if grad:
-                y = _LinearAct.apply(_LinearAct.apply(h, self.ws1, "swiglu", None), self.ws2, "none", y)
+                y = _LinearAct.apply(_LinearAct.apply(h, ws1, "swiglu", None), ws2, "none", y)
             else:
-                y = block.linear_act(block.linear_act(h, self.ws1, act="swiglu"), self.ws2, residual=y)
+                y = block.linear_act(block.linear_act(h, ws1, act="swiglu"), ws2, residual=y)
         if not norm:
             return y
         if grad:
-            return _BlockNormOut.apply(y, skip, self.norm_out, self.block_gate, scale, eps)
-        return block.block_norm_out(y, x, self.norm_out, gate=self.block_gate, residual_scale=scale, eps=eps)[0]
+            return _BlockNormOut.apply(y, skip, n2, gate, scale, eps)
+        return block.block_norm_out(y, x, n2, gate=gate, residual_scale=scale, eps=eps)[0]
 
     def _routed(self, x, logits=None, return_intermediates: bool = False):
         if return_intermediates:

@@ -165,6 +165,24 @@ def test_empty_batch_refusals_and_state(dev):
     assert set(smoe.SimpleMoE(64, 32, 4, 2, device=dev).state_dict()) == {"w_gate", "w1", "w2"}
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_module_of_another_type(dev, dtype):
+    """Parameters held in another type are converted at each call: the same
+    output, and gradients that arrive in the parameters' type."""
+    m = layer(dev, 64, 32, 4, 2, recipe="bf16", shared_intermediate=32, block_norm=True)
+    x = rand((30, 64), 9).to(BF16).to(dev)
+    with torch.no_grad():
+        want = m(x)
+        gate = m.w_gate.detach().clone()
+        m.to(dtype)
+        m.w_gate = torch.nn.Parameter(gate)
+        # fp32 holds every bf16 value, fp16 those of 2^-17 and above: what the
+        # few smaller ones of these seeded weights lose is below the output's bits
+        assert m(x).equal(want)
+    m(x).sum().backward()
+    assert all(p.grad is not None and p.grad.dtype == p.dtype for p in m.parameters())
+
+
 def test_inference_in_a_graph(dev):
     """A captured forward of the whole block, replayed on new tokens with eager
     calls in between, gives the eager bits each time."""
