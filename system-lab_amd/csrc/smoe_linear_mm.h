@@ -34,7 +34,8 @@
 // Bound by the matrix unit at the clock that the chip's power leaves it: 8192^3
 // 780 us (1409 TFLOP/s), dx 784, dW 835; 8192 x 4096 x 14336 700 (1374).  With
 // experts by their last tiles' empty rows and, in dW, by few steps a tile:
-// 65536 rows over 128 experts, 2048 x 1536, 478, dx 466, dW 580.
+// 65536 rows over 128 experts, 2048 x 1536, 462, dx 454, dW 580.  (Boxes differ by
+// 7%; the library's product took 697 to 755 for 8192^3 on them.)
 //
 // Terms past the end of the sum (K % 64, an expert's last rows) are loaded
 // from a 16-byte zero for both operands.  Rows and columns past the tile's end
@@ -436,33 +437,33 @@ __global__ __launch_bounds__(C::kThreads, 2) void linear_mm_kernel(const LinArgs
       if (steps > 1) send(1, C::kABytes, C::kBBytes);
     }
   };
-  auto sum = [&] {
-#pragma unroll
-    for (int i = 0; i < kRB; ++i)
-#pragma unroll
-      for (int j = 0; j < kCB; ++j) acc[i][j] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
-    if (steps == 0) return;
-    landed(steps == 1);
-    barrier();
-    if (second) barrier();
+  // The steps of a tile.  A wave whose rows all lie past the tile's end (an
+  // expert's last tile) keeps sending and meeting the others, and reads and
+  // multiplies nothing: 478 -> 462 us for 65536 rows over 128 experts, 2048 x 1536.
+  auto run = [&](auto has_rows) __attribute__((always_inline)) {
+    constexpr bool kRows = decltype(has_rows)::value;
     uint32_t sta = 0, far = 2 * C::kABytes;  // left stages of this step and of two steps on
     for (int s = 0; s < steps; ++s) {
       const uint32_t stb = (s & 1) * C::kBBytes;
       const bool refill = s + 2 < steps;
+      if constexpr (kRows) {
 #pragma unroll
-      for (int j = 0; j < kCB; ++j) fb[0][j] = frag_b(stb, 0, j);
+        for (int j = 0; j < kCB; ++j) fb[0][j] = frag_b(stb, 0, j);
 #pragma unroll
-      for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 0, i);
+        for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 0, i);
 #pragma unroll
-      for (int j = 0; j < kCB; ++j) fb[1][j] = frag_b(stb, 1, j);
+        for (int j = 0; j < kCB; ++j) fb[1][j] = frag_b(stb, 1, j);
+      }
       __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);  // lgkmcnt(0) alone
       barrier();
       __builtin_amdgcn_sched_barrier(0);
-      multiply(0);
+      if constexpr (kRows) multiply(0);
       __builtin_amdgcn_sched_barrier(0);
       barrier();
+      if constexpr (kRows) {
 #pragma unroll
-      for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 1, i);
+        for (int i = 0; i < kRB; ++i) fa[i] = frag_a(sta, 1, i);
+      }
       if constexpr (kAny) {
         if (refill) put(far, stb);
         if (s + 3 < steps) fetch(s + 3);
@@ -473,13 +474,25 @@ __global__ __launch_bounds__(C::kThreads, 2) void linear_mm_kernel(const LinArgs
       else __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);
       barrier();
       __builtin_amdgcn_sched_barrier(0);
-      multiply(1);
+      if constexpr (kRows) multiply(1);
       __builtin_amdgcn_sched_barrier(0);
       if (!second) landed(!refill);
       barrier();
       far = sta;
       sta = sta == 2 * C::kABytes ? 0 : sta + C::kABytes;
     }
+  };
+  auto sum = [&](int rows) {
+#pragma unroll
+    for (int i = 0; i < kRB; ++i)
+#pragma unroll
+      for (int j = 0; j < kCB; ++j) acc[i][j] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+    if (steps == 0) return;
+    landed(steps == 1);
+    barrier();
+    if (second) barrier();
+    if (wr * kRB * 16 < rows) run(std::true_type{});
+    else run(std::false_type{});
     if (kHalves && !second) barrier();
   };
 
@@ -633,7 +646,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void linear_mm_kernel(const LinArgs
   }
   while (have) {
     const MmTile done = cur;
-    sum();
+    sum(__builtin_amdgcn_readfirstlane(done.mrows));
     tile += per;
     have = locate(tile, &cur);
     if (have) {
