@@ -351,9 +351,10 @@ static int norm_waves(int H, int vec, int pieces) {
   return w;
 }
 
-// The backward pass: up to six pieces a lane, so that rows up to 3 K 16-bit
-// values need one wave and no barrier; threads of a workgroup, rows it holds at a
-// time; and workgroups: two rows a place at least, so that the partial
+// The backward pass: up to four pieces a lane, so that rows up to 2048 16-bit
+// values need one wave and no barrier (six or eight pieces were slower, by
+// registers; two as well, by barriers); threads of a workgroup, rows it holds
+// at a time; and workgroups: two rows a place at least, so that the partial
 // rows stay a small part of the traffic, two a compute unit at most.
 constexpr int kBwdPieces = 4;
 struct NormBwdPlan {
@@ -431,11 +432,9 @@ static int norm_bwd_launch(NormBwd a, void* dweight, void* dgate_ch, hipStream_t
     if (need <= 1) SMOE_NBG(1);
     else if (need <= 2) SMOE_NBG(2);
     else if (need <= 3) SMOE_NBG(3);
-    else if (need <= 4) SMOE_NBG(4);
-    else SMOE_NBG(6);
+    else SMOE_NBG(4);
   } else if (p.threads <= 512) {
-    if (need <= 4) norm_bwd_kernel<T, 4, 512, -1><<<grid, block, lds, s>>>(a);
-    else norm_bwd_kernel<T, 6, 512, -1><<<grid, block, lds, s>>>(a);
+    norm_bwd_kernel<T, 4, 512, -1><<<grid, block, lds, s>>>(a);
   } else {
     if (need <= 4) norm_bwd_kernel<T, 4, 1024, -1><<<grid, block, lds, s>>>(a);
     else if (V == 8 || need <= 8) norm_bwd_kernel<T, 8, 1024, -1><<<grid, block, lds, s>>>(a);
