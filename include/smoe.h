@@ -15,7 +15,8 @@
  *   - the caller owns every buffer; the library allocates no device memory;
  *   - bf16 tensors are passed as uint16_t (raw bf16 bits), fp8 tensors as
  *     uint8_t holding OCP float8_e4m3fn bytes (max 448, 0x7f/0xff = NaN);
- *   - every pointer must be 16-byte aligned; E <= SMOE_MAX_EXPERTS;
+ *   - every pointer must be 16-byte aligned (the unquantised operators at the
+ *     end state their own alignment and sizes); E <= SMOE_MAX_EXPERTS;
  *   - H, I, N and C (the row length of a quantised tensor) must be multiples
  *     of 16; a GEMM's K argument is the fp8 operands' row pitch, a multiple
  *     of 128.  A dimension D that is not a multiple of 128 (GPT-OSS:
